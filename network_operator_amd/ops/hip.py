@@ -68,6 +68,14 @@ def lib() -> ctypes.CDLL:
             L.netop_shm_barrier_close.restype = None
             L.netop_shm_unlink.argtypes = [ctypes.c_char_p]
             L.netop_shm_unlink.restype = i32
+            # norm.hip: what follows a reduction (norm.py packs the parameter blocks)
+            block = ctypes.c_char_p
+            L.netop_add_rms_norm.argtypes = [block, vp]
+            L.netop_add_rms_norm.restype = i32
+            L.netop_norm_backward_parts.argtypes = [u64, i32]
+            L.netop_norm_backward_parts.restype = i32
+            L.netop_add_rms_norm_backward.argtypes = [block, vp]
+            L.netop_add_rms_norm_backward.restype = i32
             _lib = L
     return _lib
 

@@ -1,0 +1,183 @@
+"""Residual RMS norm over partial sums, its 8-bit output and its gradient (``native/hip/norm.hip``).
+
+A tensor-parallel layer ends with a sum over ranks, the residual stream's addition and a norm in
+front of the next product.  :func:`add_rms_norm` does all three in one pass over 1..8 partial sums
+(``XgmiAllReduce.all_reduce_norm`` calls it on the peers' buffers)::
+
+    h            = sum(srcs) + residual               # fp32, in list order, the residual last
+    residual_out = round(h)
+    rstd         = 1 / sqrt(mean(h**2) + eps)         # over the last dimension
+    out          = round(h * rstd * weight)           # or e4m3 codes and scales
+
+Every entry point runs on the tensors' device and that device's current stream, writes into tensors
+that the caller allocated, and raises if the library is missing.  Nothing is synchronised, allocated
+on the host or kept between calls, so the calls can be captured into a graph.
+"""
+
+from __future__ import annotations
+
+import struct
+
+from . import hip
+
+MAX_SRCS = 8
+MAX_COLS = 32768  # a row stays in the registers of one workgroup
+GROUP = 128  # columns that share a scale
+
+# native/hip/norm.hip:NormParams and NormBackwardParams
+_FORWARD = struct.Struct("=9Q9q" + "QQqQqQQQ" + "6ifi")
+_BACKWARD = struct.Struct("=QqQqQqQQQqQQQ" + "6i")
+_OVERLAP = -1
+_NO_INPUTS = [0] * (MAX_SRCS + 1)
+
+
+def _dtypes():
+    import torch
+
+    return {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+
+
+def _pitch(t, shape, dtype, what, written=False):
+    """The row stride of ``t`` in elements, after its checks."""
+    if t.dtype != dtype:
+        raise ValueError(f"{what}: expected {dtype}, got {t.dtype}")
+    if t.shape != shape:
+        raise ValueError(f"{what}: expected shape {tuple(shape)}, got {tuple(t.shape)}")
+    cols = shape[-1]
+    if len(shape) == 2:
+        pitch, inner = t.stride()
+        if inner != 1 and cols > 1:
+            raise ValueError(f"{what}: the last dimension must be contiguous")
+        if written and pitch < cols and shape[0] > 1:
+            raise ValueError(f"{what}: its rows overlap")
+    else:
+        if not t.is_contiguous():
+            raise ValueError(f"{what}: only 2-D tensors may have strides")
+        pitch = cols
+    return pitch
+
+
+def _flat(t, shape, dtypes, what):
+    if t.dtype not in dtypes:
+        raise ValueError(f"{what}: expected {' or '.join(str(d) for d in dtypes)}, got {t.dtype}")
+    if t.shape != shape:
+        raise ValueError(f"{what}: expected shape {tuple(shape)}, got {tuple(t.shape)}")
+    if not t.is_contiguous():
+        raise ValueError(f"{what}: must be contiguous")
+
+
+def _on_one_device(device, tensors):
+    if device < 0 or any(t is not None and t.get_device() != device for t in tensors):
+        raise ValueError("every tensor must be on one CUDA device")
+
+
+def _checked(rc, what):
+    if rc == _OVERLAP:
+        raise ValueError("an output overlaps another tensor of the call (an output may replace an input of its type "
+                         "element on element, and nothing else)")
+    hip._check(rc, what)
+
+
+def add_rms_norm(srcs, weight, out, *, residual=None, residual_out=None, rstd=None, scales=None, eps=1e-6) -> None:
+    """The sum of 1..8 partial sums and the residual, normalised over the last dimension.
+
+    ``srcs`` (a list), ``residual`` and ``residual_out`` have ``out``'s shape ``(..., cols)`` with
+    ``cols`` up to 32768, and one type: fp32, bf16 or fp16.  2-D tensors may have any row stride (a
+    residual or partial sum with stride 0 is one row for all), others are contiguous.  ``weight``:
+    ``(cols,)`` of that type or fp32.
+
+    ``residual_out``, where given, takes the rounded sum, the next layer's residual and what the
+    backward pass needs; ``rstd`` (fp32, shape ``(...)``) the reciprocal root mean square.  Either
+    and ``out`` may be one of the inputs itself (same memory, same strides), no other overlap.
+
+    ``out`` has the inputs' type, or is ``float8_e4m3fn`` with ``scales`` (fp32): of shape ``(...)``
+    for one scale a row, or ``(..., ceil(cols / 128))`` for one a group of 128 columns.  A scale is
+    the largest magnitude / 448 (zero, with all codes zero, where that is below 2**-100); codes are
+    rounded to nearest even; ``code * scale`` is the value.
+
+    Sums and statistics are fp32; ``out`` comes from the unrounded sum and is rounded once.  An
+    infinity or NaN in a row makes that row (in 8 bits: its scale) NaN or infinite and no other.
+    """
+    import torch
+
+    kinds = _dtypes()
+    if not 1 <= len(srcs) <= MAX_SRCS:
+        raise ValueError(f"1..{MAX_SRCS} partial sums")
+    dtype, shape, device = srcs[0].dtype, out.shape, out.get_device()
+    if dtype not in kinds:
+        raise ValueError(f"partial sums: expected fp32, bf16 or fp16, got {dtype}")
+    if not shape or not 1 <= shape[-1] <= MAX_COLS:
+        raise ValueError(f"out: expected (..., cols) with 1..{MAX_COLS} columns, got shape {tuple(shape)}")
+    if not eps >= 0:
+        raise ValueError("eps must not be negative")
+    cols = shape[-1]
+    rows = out.numel() // cols
+    kind, groups = 0, shape[:-1]
+    if out.dtype == torch.float8_e4m3fn:
+        if scales is None:
+            raise ValueError("an e4m3 output needs scales")
+        kind = 1 if scales.dim() == len(groups) else 2
+        _flat(scales, groups if kind == 1 else groups + (-(-cols // GROUP),), (torch.float32,), "scales")
+    elif scales is not None:
+        raise ValueError("scales belong to an e4m3 output")
+    out_pitch = _pitch(out, shape, out.dtype if kind else dtype, "out", True)
+    ptrs, pitches = [], []
+    for t in srcs:
+        pitches.append(_pitch(t, shape, dtype, "partial sum"))
+        ptrs.append(t.data_ptr())
+    if residual is not None:
+        pitches.append(_pitch(residual, shape, dtype, "residual"))
+        ptrs.append(residual.data_ptr())
+    h_pitch = 0 if residual_out is None else _pitch(residual_out, shape, dtype, "residual_out", True)
+    _flat(weight, (cols,), (dtype, torch.float32), "weight")
+    if rstd is not None:
+        _flat(rstd, groups, (torch.float32,), "rstd")
+    _on_one_device(device, (*srcs, weight, residual, residual_out, rstd, scales))
+    if rows == 0:
+        return
+    n = len(ptrs)
+    pad = _NO_INPUTS[n:]
+    block = _FORWARD.pack(*ptrs, *pad, *pitches, *pad, weight.data_ptr(), out.data_ptr(), out_pitch,
+                          0 if residual_out is None else residual_out.data_ptr(), h_pitch,
+                          0 if rstd is None else rstd.data_ptr(), 0 if scales is None else scales.data_ptr(), rows,
+                          cols, n, kinds[dtype], weight.dtype == torch.float32, kind, device, eps, 0)
+    _checked(hip.lib().netop_add_rms_norm(block, hip._stream(out)), "netop_add_rms_norm")
+
+
+def add_rms_norm_backward(dy, h, weight, rstd, dh, dweight, *, dresidual=None) -> None:
+    """The gradient of :func:`add_rms_norm` (with an output of the inputs' type).
+
+    ``h`` is its ``residual_out`` and ``rstd`` its ``rstd``; ``dy`` the gradient of ``out``,
+    ``dresidual``, where given, that of ``residual_out``.  ``dh`` takes the gradient of the sum, which
+    is that of each partial sum and of the residual (for one that was a row for all: its rows' sum),
+    and may be ``dy``, ``h`` or ``dresidual`` itself.  ``dweight`` (``(cols,)``, the weight's type or
+    fp32) takes the weight's gradient, summed over the rows in fp32 in an order that depends on the
+    shape alone: the same inputs give the same bits.
+    """
+    import torch
+
+    kinds = _dtypes()
+    dtype, shape, device = dy.dtype, dy.shape, dy.get_device()
+    if dtype not in kinds:
+        raise ValueError(f"dy: expected fp32, bf16 or fp16, got {dtype}")
+    if not shape or not 1 <= shape[-1] <= MAX_COLS:
+        raise ValueError(f"dy: expected (..., cols) with 1..{MAX_COLS} columns, got shape {tuple(shape)}")
+    cols = shape[-1]
+    rows = dy.numel() // cols
+    dy_pitch = _pitch(dy, shape, dtype, "dy")
+    h_pitch = _pitch(h, shape, dtype, "h")
+    dh_pitch = _pitch(dh, shape, dtype, "dh", True)
+    dres_pitch = 0 if dresidual is None else _pitch(dresidual, shape, dtype, "dresidual")
+    _flat(weight, (cols,), (dtype, torch.float32), "weight")
+    _flat(rstd, shape[:-1], (torch.float32,), "rstd")
+    _flat(dweight, (cols,), (weight.dtype, torch.float32), "dweight")
+    _on_one_device(device, (h, dresidual, weight, rstd, dh, dweight))
+    L = hip.lib()
+    parts = L.netop_norm_backward_parts(rows, cols)
+    partial = torch.empty(parts * cols, dtype=torch.float32, device=dy.device)
+    block = _BACKWARD.pack(dy.data_ptr(), dy_pitch, h.data_ptr(), h_pitch,
+                           0 if dresidual is None else dresidual.data_ptr(), dres_pitch, weight.data_ptr(),
+                           rstd.data_ptr(), dh.data_ptr(), dh_pitch, dweight.data_ptr(), partial.data_ptr(), rows,
+                           cols, parts, kinds[dtype], weight.dtype == torch.float32, dweight.dtype == torch.float32,
+                           device)
+    _checked(L.netop_add_rms_norm_backward(block, hip._stream(dy)), "netop_add_rms_norm_backward")

@@ -1,0 +1,409 @@
+"""The residual RMS norm over partial sums (ops/norm.py) against its definition in 64 bits.
+
+Tolerances count roundings: half a step of the output's type, and per fp32 operation 2^-24 of the
+magnitudes that went into it."""
+
+import re
+
+import pytest
+
+torch = pytest.importorskip("torch")
+
+from network_operator_amd.ops import norm  # noqa: E402
+
+F32, BF16, F16 = torch.float32, torch.bfloat16, torch.float16
+E4M3 = torch.float8_e4m3fn
+ULP = 2.0 ** -24
+
+
+def _inputs(rows, cols, srcs, dtype, dev, residual=True, weight_dtype=None, seed=0):
+    g = torch.Generator().manual_seed(seed)
+    xs = [(torch.randn(rows, cols, generator=g) * 0.5).to(dtype).to(dev) for _ in range(srcs)]
+    res = (torch.randn(rows, cols, generator=g) * 2).to(dtype).to(dev) if residual else None
+    w = (1 + torch.randn(cols, generator=g) * 0.1).to(weight_dtype or dtype).to(dev)
+    return xs, res, w
+
+
+def _reference(xs, res, w, eps=1e-6):
+    """h, sum of magnitudes, rstd, y in 64 bits on the CPU."""
+    parts = [x.double().cpu() for x in xs] + ([] if res is None else [res.double().cpu()])
+    h = sum(parts)
+    mag = sum(p.abs() for p in parts)
+    rstd = (h.square().mean(-1) + eps).rsqrt()
+    return h, mag, rstd, h * rstd[..., None] * w.double().cpu()
+
+
+def _close(got, want, tol):
+    off = (got.double().cpu() - want).abs()
+    assert bool((off <= tol).all()), f"off by {float((off - tol).max())} more than allowed, {int((off > tol).sum())} values"
+
+
+def _check(xs, res, w, h_out, rstd_out, out, scales=None, eps=1e-6):
+    n = len(xs) + (res is not None)
+    h, mag, rstd, y = _reference(xs, res, w, eps)
+    step = torch.finfo(xs[0].dtype).eps / 2
+    cols = h.shape[-1]
+    h_err = n * ULP * mag
+    if h_out is not None:
+        _close(h_out, h, h_err + step * (h.abs() + h_err))
+    # mean of squares: each h's error, and at most 32 + 6 + 16 + 4 additions one after another
+    ss_rel = (2 * (h.abs() * h_err).sum(-1) / h.square().sum(-1).clamp(min=1e-300) + 64 * ULP).clamp(max=1)
+    r_err = rstd * (ss_rel / 2 + 4 * ULP)
+    if rstd_out is not None:
+        _close(rstd_out, rstd, r_err)
+    wa = w.double().cpu().abs()
+    y_err = wa * (h_err * rstd[..., None] + h.abs() * r_err[..., None]) * 1.01 + 4 * ULP * y.abs()
+    if scales is None:
+        _close(out, y, y_err + step * (y.abs() + y_err) + torch.finfo(xs[0].dtype).smallest_normal * step)
+        return
+    s = scales.double().cpu()
+    per = s[..., None] if s.dim() == h.dim() - 1 else s.repeat_interleave(norm.GROUP, -1)[..., :cols]
+    width = cols if s.dim() == h.dim() - 1 else norm.GROUP
+    amax = torch.nn.functional.pad(y.abs(), (0, -cols % width)).unflatten(-1, (-1, width)).amax(-1)
+    err = torch.nn.functional.pad(y_err, (0, -cols % width)).unflatten(-1, (-1, width)).amax(-1)
+    _close(s.view(amax.shape), amax / 448, err / 448 + 2 * ULP * amax / 448)
+    # half a step of e4m3: 2^-4 of the value, 2^-10 of the scale among the smallest
+    half = torch.maximum(y.abs() * 2.0 ** -4, per * 2.0 ** -10)
+    _close(out.float().cpu().double() * per, y, half * (1 + 8 * ULP) + 2 * y_err + 8 * ULP * y.abs())
+
+
+def _empty_like_case(shape, dtype, kind, dev):
+    cols = shape[-1]
+    if kind == "same":
+        return torch.empty(shape, dtype=dtype, device=dev), None
+    s = shape[:-1] if kind == "row" else shape[:-1] + (-(-cols // norm.GROUP),)
+    return torch.empty(shape, dtype=E4M3, device=dev), torch.empty(s, dtype=F32, device=dev)
+
+
+# ---- refusals (no GPU) ------------------------------------------------------------------------
+def _cpu_call(**kw):
+    c = dict(rows=4, cols=16, dtype=BF16)
+    x = torch.zeros(c["rows"], c["cols"], dtype=c["dtype"])
+    a = dict(srcs=[x.clone()], weight=torch.ones(c["cols"], dtype=c["dtype"]), out=x.clone())
+    a.update(kw)
+    return norm.add_rms_norm(a.pop("srcs"), a.pop("weight"), a.pop("out"), **a)
+
+
+@pytest.mark.parametrize("kw,why", [
+    (dict(srcs=[]), "1..8 partial sums"),
+    (dict(srcs=[torch.zeros(4, 16, dtype=BF16)] * 9), "1..8 partial sums"),
+    (dict(srcs=[torch.zeros(4, 16, dtype=torch.float64)]), "expected fp32, bf16 or fp16"),
+    (dict(srcs=[torch.zeros(4, 16, dtype=BF16), torch.zeros(4, 16)]), "expected torch.bfloat16"),
+    (dict(srcs=[torch.zeros(4, 8, dtype=BF16)]), "expected shape"),
+    (dict(out=torch.zeros(4, 16)), "expected torch.bfloat16"),
+    (dict(out=torch.zeros(4, 0, dtype=BF16), srcs=[torch.zeros(4, 0, dtype=BF16)]), "columns"),
+    (dict(out=torch.zeros(1, 32769, dtype=BF16), srcs=[torch.zeros(1, 32769, dtype=BF16)]), "columns"),
+    (dict(out=torch.zeros((), dtype=BF16)), "columns"),
+    (dict(out=torch.zeros(4, 16).to(E4M3)), "needs scales"),
+    (dict(scales=torch.zeros(4)), "belong to an e4m3 output"),
+    (dict(out=torch.zeros(4, 16).to(E4M3), scales=torch.zeros(5)), "expected shape"),
+    (dict(out=torch.zeros(4, 16).to(E4M3), scales=torch.zeros(4, 2)), "expected shape"),
+    (dict(out=torch.zeros(4, 16).to(E4M3), scales=torch.zeros(4, dtype=BF16)), "scales: expected torch.float32"),
+    (dict(weight=torch.ones(8, dtype=BF16)), "weight: expected shape"),
+    (dict(weight=torch.ones(16, dtype=F16)), "weight: expected"),
+    (dict(residual=torch.zeros(4, 16)), "residual: expected torch.bfloat16"),
+    (dict(residual=torch.zeros(16, 4, dtype=BF16).t()), "last dimension must be contiguous"),
+    (dict(residual_out=torch.zeros(1, 16, dtype=BF16).expand(4, 16)), "rows overlap"),
+    (dict(rstd=torch.zeros(5)), "rstd: expected shape"),
+    (dict(rstd=torch.zeros(4, dtype=BF16)), "rstd: expected torch.float32"),
+    (dict(eps=-1.0), "eps"),
+    (dict(eps=float("nan")), "eps"),
+    (dict(), "one CUDA device"),
+])
+def test_forward_refuses(kw, why):
+    with pytest.raises(ValueError, match=re.escape(why)):
+        _cpu_call(**kw)
+
+
+def test_backward_refuses():
+    x = torch.zeros(4, 16, dtype=BF16)
+    w, rstd, dw = torch.ones(16, dtype=BF16), torch.ones(4), torch.zeros(16)
+    good = dict(dy=x, h=x.clone(), weight=w, rstd=rstd, dh=x.clone(), dweight=dw)
+    for kw, why in [(dict(h=x.float()), "h: expected"), (dict(rstd=rstd[:3]), "rstd: expected shape"),
+                    (dict(dy=x.double()), "expected fp32, bf16 or fp16"), (dict(weight=w[:8]), "weight: expected shape"),
+                    (dict(dweight=dw[:8]), "dweight: expected shape"), (dict(dweight=dw.to(F16)), "dweight: expected"),
+                    (dict(dresidual=x[:2]), "dresidual: expected shape"), (dict(dh=x[:1].expand(4, 16)), "rows overlap"),
+                    (dict(dh=x.t().contiguous().t()), "last dimension must be contiguous"), (dict(), "one CUDA device")]:
+        with pytest.raises(ValueError, match=re.escape(why)):
+            norm.add_rms_norm_backward(**{**good, **kw})
+
+
+@pytest.mark.gpu
+def test_overlaps_are_refused_and_columns_of_one_buffer_are_not(cuda_device):
+    buf = torch.randn(6, 64, device=cuda_device).to(BF16)
+    w = torch.ones(16, dtype=BF16, device=cuda_device)
+    x, res, out, h = (buf[:4, i * 16:(i + 1) * 16] for i in range(4))
+    norm.add_rms_norm([x], w, out, residual=res, residual_out=h)
+    _check([x], res, w, h, None, out)
+    for kw in (dict(out=buf[1:5, :16]), dict(out=buf[:4, 8:24]), dict(out=out, residual_out=out),
+               dict(out=buf.view(-1)[8:8 + 64].view(4, 16))):
+        o = kw.pop("out")
+        with pytest.raises(ValueError, match="overlaps"):
+            norm.add_rms_norm([x], w, o, residual=res, **kw)
+    flat = torch.zeros(4 * 16, dtype=BF16, device=cuda_device)
+    with pytest.raises(ValueError, match="overlaps"):
+        norm.add_rms_norm([x], flat[:16], flat.view(4, 16))
+    one = torch.zeros(1, 16, dtype=BF16, device=cuda_device).expand(4, 16)
+    with pytest.raises(ValueError, match="overlaps"):  # an output of four rows over a row for all
+        norm.add_rms_norm([one], w, flat.as_strided((4, 16), (16, 1)), residual=flat[:16].expand(4, 16))
+
+
+# ---- forward ----------------------------------------------------------------------------------
+SHAPES = [(1, 1), (3, 7), (1, 8), (5, 64), (4, 129), (9, 512), (7, 513), (3, 1000), (2, 1024), (3, 1025), (6, 2048),
+          (2, 2051), (5, 4096), (2, 4099), (3, 5003), (2, 8192), (3, 8200), (2, 16384), (1, 16387), (2, 32768), (1, 32765)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["same", "row", "group"])
+@pytest.mark.parametrize("i,shape", list(enumerate(SHAPES)))
+def test_forward(cuda_device, i, shape, kind):
+    dtype = (BF16, F16, F32)[(i + len(kind)) % 3]
+    srcs = (1, 2, 3, 4, 5, 7, 8)[i % 7]
+    xs, res, w = _inputs(*shape, srcs, dtype, cuda_device, residual=i % 4 != 1, weight_dtype=F32 if i % 2 else None, seed=i)
+    out, scales = _empty_like_case(shape, dtype, kind, cuda_device)
+    h, rstd = torch.empty(shape, dtype=dtype, device=cuda_device), torch.empty(shape[0], device=cuda_device)
+    norm.add_rms_norm(xs, w, out, residual=res, residual_out=h, rstd=rstd, scales=scales)
+    _check(xs, res, w, h, rstd, out, scales)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("rows,cols", [(70000, 64), (5000, 1536), (600, 8192), (300, 20000)])
+def test_forward_many_rows(cuda_device, rows, cols, dtype):
+    xs, res, w = _inputs(rows, cols, 1, dtype, cuda_device, seed=rows)
+    out = torch.empty_like(xs[0])
+    norm.add_rms_norm(xs, w, out, residual=res)
+    pick = torch.tensor([0, 1, rows // 2, rows - 2, rows - 1], device=cuda_device)
+    _check([xs[0][pick]], res[pick], w, None, None, out[pick])
+    whole = xs[0].float() + res.float()  # every row within a few roundings of the same in fp32
+    y = whole * (whole.square().mean(1, keepdim=True) + 1e-6).rsqrt() * w.float()
+    assert bool(((out.float() - y).abs() <= torch.finfo(dtype).eps * y.abs() + 1e-5 * (dtype == F32) + 1e-6).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["same", "row", "group"])
+@pytest.mark.parametrize("cols,shift", [(40, 1), (257, 3), (2050, 5), (9001, 7)])
+def test_odd_strides_and_offsets_leave_the_neighbours_alone(cuda_device, cols, shift, kind):
+    """Every tensor a view at an odd offset with an odd row stride; what lies around the outputs stays."""
+    rows, pitch = 5, cols + 2 * shift + 1
+    g = torch.Generator().manual_seed(cols)
+
+    def view(dtype, fill=None):
+        buf = torch.randn(rows * pitch + shift, generator=g).to(dtype if dtype != E4M3 else F32)
+        buf = (buf if fill is None else torch.full_like(buf, fill)).to(dtype).to(cuda_device)
+        return buf, buf.as_strided((rows, cols), (pitch, 1), shift)
+
+    x, res = view(BF16)[1], view(BF16)[1]
+    w = torch.randn(cols + 1, generator=g).to(cuda_device)[1:]
+    (ob, out), (hb, h) = view(BF16 if kind == "same" else E4M3, 7.0), view(BF16, 7.0)
+    scales = _empty_like_case((rows, cols), BF16, kind, cuda_device)[1]
+    norm.add_rms_norm([x], w, out, residual=res, residual_out=h, scales=scales)
+    _check([x], res, w, h, None, out, scales)
+    for buf, t in ((ob, out), (hb, h)):
+        kept = torch.ones(buf.numel(), dtype=torch.bool, device=cuda_device)
+        kept.as_strided((rows, cols), (pitch, 1), shift).fill_(False)
+        assert bool((buf.float()[kept] == 7).all())
+
+
+@pytest.mark.gpu
+def test_shapes_other_than_two_dimensions_and_no_rows(cuda_device):
+    for shape in [(24,), (2, 3, 40), (2, 1, 3, 8)]:
+        x = torch.randn(shape, device=cuda_device)
+        w, out, rstd = torch.rand(shape[-1], device=cuda_device), torch.empty_like(x), torch.empty(shape[:-1], device=cuda_device)
+        norm.add_rms_norm([x], w, out, rstd=rstd)
+        _check([x], None, w, None, rstd, out)
+    x = torch.empty(0, 24, dtype=BF16, device=cuda_device)
+    w, dw = torch.ones(24, dtype=BF16, device=cuda_device), torch.full((24,), 5.0, device=cuda_device)
+    norm.add_rms_norm([x], w, x.clone())
+    norm.add_rms_norm_backward(x, x, w, torch.empty(0, device=cuda_device), x.clone(), dw)
+    assert bool((dw == 0).all())
+    with pytest.raises(ValueError, match="2-D"):
+        y = torch.zeros(2, 3, 16, device=cuda_device).transpose(0, 1)
+        norm.add_rms_norm([y], torch.ones(16, device=cuda_device), torch.zeros(3, 2, 16, device=cuda_device))
+
+
+@pytest.mark.gpu
+def test_a_row_for_all_and_outputs_in_place(cuda_device):
+    xs, res, w = _inputs(6, 1000, 2, BF16, cuda_device, seed=3)
+    bias = torch.randn(1000, device=cuda_device).to(BF16)
+    out = torch.empty_like(res)
+    norm.add_rms_norm(xs, w, out, residual=bias.expand(6, 1000))
+    _check(xs, bias.expand(6, 1000), w, None, None, out)
+    x0, r0 = xs[0].clone(), res.clone()
+    norm.add_rms_norm(xs, w, xs[0], residual=res, residual_out=res)
+    _check([x0, xs[1]], r0, w, res, None, xs[0])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["same", "row", "group"])
+def test_infinities_nan_and_zeros_stay_in_their_row(cuda_device, kind):
+    xs, res, w = _inputs(6, 300, 1, BF16, cuda_device, seed=4)
+    x = xs[0]
+    x[1, 7], x[2, 299], x[4] = float("inf"), float("nan"), 0
+    res[4] = 0
+    out, scales = _empty_like_case((6, 300), BF16, kind, cuda_device)
+    norm.add_rms_norm(xs, w, out, residual=res, scales=scales)
+    fine = torch.tensor([0, 3, 5], device=cuda_device)
+    _check([x[fine]], res[fine], w, None, None, out.float()[fine].to(out.dtype), None if scales is None else scales[fine])
+    assert bool((out[4].float() == 0).all())
+    bad = out.float() if scales is None else scales
+    assert not bool(torch.isfinite(bad[1]).all()) and not bool(torch.isfinite(bad[2]).all())
+    if scales is not None:
+        assert bool((scales[4] == 0).all())
+
+
+@pytest.mark.gpu
+def test_tiny_and_huge_rows(cuda_device):
+    """Rows whose squares lie at the edges of fp32: eps rules the small ones, scales stay exact."""
+    x = torch.randn(4, 512, device=cuda_device)
+    x[0] *= 1e-20
+    x[1] *= 1e15
+    x[2] *= 1e-3
+    w = torch.full((512,), 1e-28, device=cuda_device)
+    out, scales = _empty_like_case((4, 512), F32, "row", cuda_device)
+    norm.add_rms_norm([x], w, out, scales=scales)
+    assert float(scales[0]) == 0 and bool((out[0].float() == 0).all())  # below 2^-100
+    _check([x[1:]], None, w, None, None, out.float()[1:].to(E4M3), scales[1:])
+
+
+@pytest.mark.gpu
+def test_row_offsets_pass_32_bits(cuda_device):
+    pitch = (1 << 31) + 8  # elements; row 2 starts 8 GiB in
+    free, _ = torch.cuda.mem_get_info(cuda_device)
+    if free < 24 << 30:
+        pytest.skip("needs 24 GiB")
+    buf = torch.empty(2 * pitch + 4096, dtype=BF16, device=cuda_device)
+    x = buf.as_strided((3, 4096), (pitch, 1))
+    try:
+        x.copy_(torch.randn(3, 4096))
+        x0, w, rstd = x.clone(), torch.rand(4096, device=cuda_device).to(BF16), torch.empty(3, device=cuda_device)
+        norm.add_rms_norm([x], w, x, rstd=rstd)
+        _check([x0], None, w, None, rstd, x)
+        dy, dw = torch.randn(3, 4096, device=cuda_device).to(BF16), torch.empty(4096, device=cuda_device)
+        x.copy_(x0)
+        want = torch.empty_like(dy)
+        norm.add_rms_norm_backward(dy, x0, w, rstd, want, dw)
+        norm.add_rms_norm_backward(dy, x, w, rstd, x, dw)
+        assert torch.equal(x, want)
+    finally:
+        del buf, x
+        torch.cuda.empty_cache()
+
+
+# ---- backward ---------------------------------------------------------------------------------
+def _gradient(dy, h, w, rstd, dres):
+    dy, h, w, r = (t.double().cpu() for t in (dy, h, w, rstd))
+    r = r[..., None]
+    a = dy * w
+    dot = (a * h).mean(-1, keepdim=True)
+    dh = r * a - h * r ** 3 * dot
+    mag = r * a.abs() + h.abs() * r ** 3 * (a * h).abs().mean(-1, keepdim=True)
+    if dres is not None:
+        dh, mag = dh + dres.double().cpu(), mag + dres.double().cpu().abs()
+    return dh, mag, (dy * h * r).flatten(0, -2).sum(0), (dy * h * r).abs().flatten(0, -2).sum(0)
+
+
+def _check_backward(dy, h, w, rstd, dres, dh, dw):
+    want, mag, dw_want, dw_mag = _gradient(dy, h, w, rstd, dres)
+    # the dot product: at most 64 additions one after another; a few products on the way
+    _close(dh, want, torch.finfo(dh.dtype).eps / 2 * want.abs() * 1.001 + 80 * ULP * mag
+           + torch.finfo(dh.dtype).smallest_normal * 2.0 ** -8)
+    rows = dy.numel() // dy.shape[-1]
+    parts = max(1, min(rows, 1024))
+    adds = rows / parts + parts / 32 + 32 + 4
+    _close(dw, dw_want, torch.finfo(dw.dtype).eps / 2 * dw_want.abs() * 1.001 + adds * ULP * dw_mag + 1e-30)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("i,shape", list(enumerate(SHAPES + [(3000, 64), (1500, 520), (2100, 4096), (1100, 9000)])))
+def test_backward(cuda_device, i, shape):
+    dtype = (F16, F32, BF16)[i % 3]
+    g = torch.Generator().manual_seed(i)
+    dy, h, dres = ((torch.randn(shape, generator=g) * s).to(dtype).to(cuda_device) for s in (0.1, 2, 0.1))
+    w = (1 + torch.randn(shape[-1], generator=g) * 0.1).to(F32 if i % 2 else dtype).to(cuda_device)
+    rstd = h.float().square().mean(-1).add(1e-6).rsqrt()
+    dres = None if i % 4 == 2 else dres
+    dh, dw = torch.empty_like(dy), torch.empty(shape[-1], dtype=F32 if i % 5 else w.dtype, device=cuda_device)
+    norm.add_rms_norm_backward(dy, h, w, rstd, dh, dw, dresidual=dres)
+    _check_backward(dy, h, w, rstd, dres, dh, dw)
+    again, dw2 = dy.clone(), torch.empty_like(dw)
+    norm.add_rms_norm_backward(again, h, w, rstd, again, dw2, dresidual=dres)  # in place, the same bits
+    assert torch.equal(again, dh) and torch.equal(dw2, dw)
+
+
+@pytest.mark.gpu
+def test_gradient_against_differences(cuda_device):
+    """Along a random direction of every input: differences of the definition in 64 bits."""
+    xs, res, w = _inputs(5, 203, 3, F32, cuda_device, seed=9)
+    h, rstd, out = torch.empty_like(res), torch.empty(5, device=cuda_device), torch.empty_like(res)
+    norm.add_rms_norm(xs, w, out, residual=res, residual_out=h, rstd=rstd)
+    g = torch.Generator().manual_seed(1)
+    dy, dres, direction = (torch.randn(5, 203, generator=g).double() for _ in range(3))
+    wdir = torch.randn(203, generator=g).double()
+    dh, dw = torch.empty_like(res), torch.empty_like(w)
+    norm.add_rms_norm_backward(dy.float().to(cuda_device), h, w, rstd, dh, dw, dresidual=dres.float().to(cuda_device))
+    dy, dres = dy.float().double(), dres.float().double()
+
+    def f(k, t):  # the k-th input moved by t along the direction
+        moved = [x.double().cpu() for x in (*xs, res)]
+        weight = w.double().cpu()
+        if k < 4:
+            moved[k] = moved[k] + t * direction
+        else:
+            weight = weight + t * wdir
+        hh, _, _, y = _reference(moved[:3], moved[3], weight)
+        return float((dy * y).sum() + (dres * hh).sum())
+
+    e = 1e-5
+    for k in range(5):
+        want = (f(k, e) - f(k, -e)) / (2 * e)
+        got = float((dh.double().cpu() * direction).sum()) if k < 4 else float((dw.double().cpu() * wdir).sum())
+        # 1015 products of fp32 results, each off by some 100 roundings of a value of about one
+        assert abs(got - want) <= 100 * ULP * 1015 + 1e-6 * abs(want)
+
+
+@pytest.mark.gpu
+def test_backward_refuses_overlaps_and_mixed_devices(cuda_device):
+    x = torch.zeros(4, 16, dtype=BF16, device=cuda_device)
+    w, rstd, dw = torch.ones(16, device=cuda_device), torch.ones(4, device=cuda_device), torch.zeros(16, device=cuda_device)
+    buf = torch.zeros(5, 16, dtype=BF16, device=cuda_device)
+    good = dict(dy=x, h=buf[:4], weight=w, rstd=rstd, dh=x.clone(), dweight=dw)
+    for kw, why in [(dict(dweight=w), "overlaps"), (dict(dh=buf[1:]), "overlaps"), (dict(h=x.cpu()), "one CUDA device"),
+                    (dict(rstd=rstd.cpu()), "one CUDA device")]:
+        with pytest.raises(ValueError, match=why):
+            norm.add_rms_norm_backward(**{**good, **kw})
+
+
+# ---- streams and graphs -----------------------------------------------------------------------
+@pytest.mark.gpu
+def test_side_stream_and_captured_graph(cuda_device):
+    """Forward and backward captured together, replayed with eager work and other inputs between."""
+    xs, res, w = _inputs(64, 2048, 4, BF16, cuda_device, seed=5)
+    out, h, rstd = torch.empty_like(res), torch.empty_like(res), torch.empty(64, device=cuda_device)
+    q, scales = _empty_like_case((64, 2048), BF16, "row", cuda_device)
+    dh, dw = torch.empty_like(res), torch.empty(2048, device=cuda_device)
+
+    def passes():
+        norm.add_rms_norm(xs, w, out, residual=res, residual_out=h, rstd=rstd)
+        norm.add_rms_norm(xs, w, q, residual=res, scales=scales)
+        norm.add_rms_norm_backward(out, h, w, rstd, dh, dw, dresidual=h)
+
+    side = torch.cuda.Stream(device=cuda_device)
+    side.wait_stream(torch.cuda.current_stream(cuda_device))
+    with torch.cuda.stream(side):
+        passes()
+    side.synchronize()
+    _check(xs, res, w, h, rstd, out)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        passes()
+    for seed in range(4):
+        new, _, _ = _inputs(64, 2048, 4, BF16, cuda_device, seed=20 + seed)
+        for x, y in zip(xs, new):
+            x.copy_(y)
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [t.clone() for t in (out, h, rstd, q.view(torch.uint8), scales, dh, dw)]
+        passes()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, (out, h, rstd, q.view(torch.uint8), scales, dh, dw)))

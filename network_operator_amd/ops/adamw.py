@@ -1,0 +1,295 @@
+"""The optimizer's side of a data-parallel step: the global gradient norm and AdamW over many
+tensors at once (``native/hip/adamw.hip``), for gradients that an all-reduce has summed (the hooks
+of ``parallel/ddp_hooks.py``; ``parallel/sharded_adamw.py`` composes both with the reduce-scatter)::
+
+    opt = AdamW(params, lr=3e-4, weight_decay=0.1, state_bits=8)
+    total, coef = torch.empty(1, device=dev), torch.empty(1, device=dev)
+    for step in range(1, steps + 1):
+        ...                                             # backward, all-reduce
+        grads = [p.grad for p in params]
+        grad_norm(grads, total, coef=coef, max_norm=1.0)
+        opt.step(grads, step=step, coef=coef)           # coef is read on the device
+
+Both run on the tensors' device and its current stream, without a synchronisation, and can be
+captured into a graph (``step`` and ``lr`` may be tensors there).  They raise if the library is
+missing.
+"""
+
+from __future__ import annotations
+
+import math
+import struct
+from array import array
+
+from . import hip
+
+BLOCK = 256  # elements of a tensor that share a scale; every tensor's states start at a whole block
+
+# native/hip/adamw.hip:Hyper and StepParams
+_HYPER = struct.Struct("=9fI")
+_STEP = struct.Struct("=8Q" + "9fI" + "6i")
+
+
+def _dtypes():
+    import torch
+
+    return {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+
+
+def _one(t, dtype, device, what):
+    if t.dtype != dtype or t.numel() != 1:
+        raise ValueError(f"{what}: expected one {dtype} element")
+    if t.get_device() != device:
+        raise ValueError("every tensor must be on one CUDA device")
+    return t.data_ptr()
+
+
+def grad_norm(grads, total, *, norms=None, coef=None, max_norm=None, scale=1.0) -> None:
+    """The 2-norm of all ``grads`` together, times ``scale`` (1 / ranks for summed gradients).
+
+    ``grads``: contiguous tensors of one type (fp32, bf16 or fp16); ``None`` counts as zeros.
+    ``total`` (fp32, one element) takes the norm; ``norms`` (fp32, one a gradient), where given, each
+    gradient's own, times ``scale`` too; ``coef`` (fp32, one element), where given,
+    ``scale * min(1, max_norm / (total + 1e-6))``, the factor :meth:`AdamW.step` takes (``scale``
+    without ``max_norm``).  Where the norm is infinite or NaN ``coef`` is NaN, and that step is left out.
+
+    Squares are summed in 64 bits, in an order that depends on the sizes alone: no gradient is too
+    large or too small, and the same inputs give the same bits.
+    """
+    import torch
+
+    kinds = _dtypes()
+    first = next((g for g in grads if g is not None), None)
+    if first is None:
+        raise ValueError("no gradients")
+    dtype, device = first.dtype, first.get_device()
+    if dtype not in kinds:
+        raise ValueError(f"gradients: expected fp32, bf16 or fp16, got {dtype}")
+    limit = math.inf if max_norm is None else float(max_norm)
+    if not limit >= 0:
+        raise ValueError("max_norm must not be negative")
+    if not math.isfinite(scale):
+        raise ValueError("scale must be finite")
+    ptrs, ns = array("Q"), array("Q")
+    for g in grads:
+        if g is None:
+            ptrs.append(0)
+            ns.append(0)
+            continue
+        if g.dtype != dtype:
+            raise ValueError(f"gradients must have one type: {dtype} and {g.dtype}")
+        if not g.is_contiguous():
+            raise ValueError("gradients must be contiguous")
+        if g.get_device() != device:
+            raise ValueError("every tensor must be on one CUDA device")
+        ptrs.append(g.data_ptr())
+        ns.append(g.numel())
+    total_ptr = _one(total, torch.float32, device, "total")
+    coef_ptr = 0 if coef is None else _one(coef, torch.float32, device, "coef")
+    norms_ptr = 0
+    if norms is not None:
+        if norms.dtype != torch.float32 or norms.shape != (len(ns),) or not norms.is_contiguous():
+            raise ValueError(f"norms: expected {len(ns)} contiguous float32 elements")
+        if norms.get_device() != device:
+            raise ValueError("every tensor must be on one CUDA device")
+        norms_ptr = norms.data_ptr()
+    if device < 0:
+        raise ValueError("every tensor must be on one CUDA device")
+    elements = sum(ns)
+    stretch = 1 << 13  # elements a workgroup: enough of them to fill the chip, few enough to add up
+    while stretch < 1 << 16 and elements // stretch > 4096:
+        stretch *= 2
+    stretches = elements // stretch + len(ns)
+    work = torch.empty(stretches + len(ns), dtype=torch.float64, device=first.device)
+    hip._check(hip.lib().netop_grad_norm(ptrs.buffer_info()[0], ns.buffer_info()[0], len(ns), kinds[dtype], stretch,
+                                         work.data_ptr(), stretches, total_ptr, norms_ptr, coef_ptr, scale, limit,
+                                         device, hip._stream(first)), "netop_grad_norm")
+
+
+class AdamW:
+    """AdamW over ``params`` (contiguous CUDA tensors of one type and device), with its states::
+
+        g' = scale * coef * g
+        m  = b1 m + (1 - b1) g'          v = b2 v + (1 - b2) g'^2
+        p  = p (1 - lr wd) - lr (m / (1 - b1^step)) / (sqrt(v / (1 - b2^step)) + eps)
+
+    fp32 parameters are updated in place.  bf16 and fp16 parameters are roundings of fp32 masters kept
+    here (``master``, from the parameters' values at first): a step is mostly smaller than half a step
+    of their own.
+
+    ``state_bits=32`` keeps ``exp_avg`` (m) and ``exp_avg_sq`` (v) in fp32.  ``state_bits=8`` keeps
+    m and sqrt(v) as e4m3 codes with one fp32 scale a block of 256 elements of a tensor
+    (``exp_avg_scale``, ``exp_avg_sq_scale``; value = code * scale, v its square).  They are rounded
+    up or down at random, in proportion, from a hash of (``seed``, ``step``, position): the same seed
+    gives the same bits.  A sqrt(v) other than zero stays other than zero; a block whose m all lie
+    below 2**-100 becomes zeros.
+
+    All states are flat, with each tensor at a multiple of 256 elements (``offsets``); what lies
+    between is zero.  The parameters must stay where they are: a step on one that has moved (``.data``
+    replaced, ``module.to``) raises.  Steps on one object follow each other on one stream, or are
+    ordered by the caller.
+    """
+
+    def __init__(self, params, *, lr, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.01, state_bits=32, seed=0):
+        import torch
+
+        kinds = _dtypes()
+        self.params = list(params)
+        if not self.params:
+            raise ValueError("no parameters")
+        first = self.params[0]
+        self.dtype, self.device = first.dtype, first.device
+        if self.dtype not in kinds:
+            raise ValueError(f"parameters: expected fp32, bf16 or fp16, got {self.dtype}")
+        if state_bits not in (8, 32):
+            raise ValueError("state_bits must be 8 or 32")
+        if not all(0 <= b < 1 for b in betas) or len(betas) != 2:
+            raise ValueError("betas must be two numbers in [0, 1)")
+        if not 1e-30 <= eps < math.inf:  # zero would make 0 / 0 of an element that never had a gradient
+            raise ValueError("eps must be positive")
+        for name, x in (("lr", lr), ("weight_decay", weight_decay)):
+            if not 0 <= x < math.inf:
+                raise ValueError(f"{name} must not be negative")
+        if not 0 <= seed < 1 << 32:
+            raise ValueError("seed must fit 32 bits")
+        for p in self.params:
+            if p.dtype != self.dtype:
+                raise ValueError(f"parameters must have one type: {self.dtype} and {p.dtype}")
+            if not p.is_contiguous():
+                raise ValueError("parameters must be contiguous")
+        held = sorted((p.data_ptr(), p.numel() * p.element_size()) for p in self.params if p.numel())
+        if any(a + n > b for (a, n), (b, _) in zip(held, held[1:])):
+            raise ValueError("two parameters share memory")
+        if not all(p.is_cuda and p.device == self.device for p in self.params):
+            raise ValueError("every tensor must be on one CUDA device")
+        self.lr, self.betas, self.eps, self.weight_decay = float(lr), tuple(betas), float(eps), float(weight_decay)
+        self.state_bits, self.seed = state_bits, seed
+        self._kind, self._index = kinds[self.dtype], first.get_device()
+        self._ptrs = [p.data_ptr() for p in self.params]
+        self._shapes = [p.shape for p in self.params]
+        ns = [p.numel() for p in self.params]
+        self.offsets, total = [], 0
+        for n in ns:
+            self.offsets.append(total)
+            total += -(-n // BLOCK) * BLOCK
+        new = dict(device=self.device)
+        codes = torch.float8_e4m3fn if state_bits == 8 else torch.float32
+        self.exp_avg = torch.zeros(total, dtype=torch.uint8 if state_bits == 8 else codes, **new).view(codes)
+        self.exp_avg_sq = torch.zeros_like(self.exp_avg.view(torch.uint8)).view(codes)
+        self.exp_avg_scale = torch.zeros(total // BLOCK, **new) if state_bits == 8 else None
+        self.exp_avg_sq_scale = torch.zeros(total // BLOCK, **new) if state_bits == 8 else None
+        self.master = None
+        if self._kind:
+            self.master = torch.zeros(total, **new)
+            for p, at, n in zip(self.params, self.offsets, ns):
+                self.master[at:at + n].copy_(p.detach().reshape(-1))
+        self._plan(ns)
+
+    def _plan(self, ns):
+        """The table of chunks, in launches of as many tensors as have room for their gradients' addresses."""
+        import torch
+
+        L = hip.lib()
+        chunk, most = L.netop_adamw_chunk(), L.netop_adamw_max_grads()
+        n = torch.tensor(ns, dtype=torch.int64)
+        count = (n + chunk - 1) // chunk
+        of = torch.repeat_interleave(torch.arange(len(ns)), count)
+        start = (torch.arange(len(of)) - (torch.cumsum(count, 0) - count)[of]) * chunk
+        table = torch.empty(len(of), 4, dtype=torch.int64)
+        table[:, 0] = torch.tensor(self._ptrs)[of] + start * self.params[0].element_size()
+        table[:, 1] = torch.tensor(self.offsets)[of] + start
+        table[:, 2] = start
+        table[:, 3] = torch.minimum(n[of] - start, torch.tensor(chunk)) | (of % most) << 32
+        self._table = table.to(self.device)
+        self._launches = []  # (first tensor, one behind the last, address of its chunks, how many)
+        at = 0
+        for a in range(0, len(ns), most):
+            c = int(count[a:a + most].sum())
+            self._launches.append((a, min(a + most, len(ns)), self._table.data_ptr() + at * 32, c))
+            at += c
+
+    def state_dict(self) -> dict:
+        """The states themselves (not copies); ``None`` for those this optimizer has not."""
+        return dict(exp_avg=self.exp_avg, exp_avg_sq=self.exp_avg_sq, master=self.master,
+                    exp_avg_scale=self.exp_avg_scale, exp_avg_sq_scale=self.exp_avg_sq_scale)
+
+    def load_state_dict(self, state: dict) -> None:
+        """Copies states in that :meth:`state_dict` of an optimizer over tensors of these sizes gave;
+        the parameters are not touched."""
+        mine = self.state_dict()
+        for k, t in mine.items():
+            x = state.get(k)
+            if (x is None) != (t is None) or t is not None and (x.shape != t.shape or x.dtype != t.dtype):
+                raise ValueError(f"{k}: expected {None if t is None else (tuple(t.shape), t.dtype)}, "
+                                 f"got {None if x is None else (tuple(x.shape), x.dtype)}")
+        for k, t in mine.items():
+            if t is not None:
+                t.copy_(state[k])
+
+    def step(self, grads, *, step, lr=None, coef=None, scale=1.0) -> None:
+        """One step from ``grads``, one a parameter: contiguous, of its shape, all of one type (fp32,
+        bf16 or fp16).  A parameter whose gradient is ``None`` is left as it is, with its states.
+
+        ``step`` counts from 1: a number, or an int64 tensor of one element on the device.  ``lr``
+        replaces the constructor's: a number, or an fp32 tensor of one element.  ``coef`` (an fp32
+        tensor of one element, from :func:`grad_norm`) and the number ``scale`` multiply the
+        gradients; where the product with ``coef`` is not finite, nothing is changed.
+        """
+        import torch
+
+        if len(grads) != len(self.params):
+            raise ValueError(f"{len(self.params)} gradients expected, got {len(grads)}")
+        if [p.data_ptr() for p in self.params] != self._ptrs:
+            raise ValueError("a parameter has moved since the optimizer was made")
+        device, gtype, ptrs = self._index, None, array("Q")
+        for g, shape in zip(grads, self._shapes):
+            if g is None:
+                ptrs.append(0)
+                continue
+            if gtype is None:
+                gtype = g.dtype
+            if g.dtype != gtype:
+                raise ValueError(f"gradients must have one type: {gtype} and {g.dtype}")
+            if g.shape != shape:
+                raise ValueError(f"a gradient of shape {tuple(g.shape)} for a parameter of shape {tuple(shape)}")
+            if not g.is_contiguous():
+                raise ValueError("gradients must be contiguous")
+            if g.get_device() != device:
+                raise ValueError("every tensor must be on one CUDA device")
+            ptrs.append(g.data_ptr())
+        if gtype is None:
+            return
+        kinds = _dtypes()
+        if gtype not in kinds:
+            raise ValueError(f"gradients: expected fp32, bf16 or fp16, got {gtype}")
+        if not math.isfinite(scale):
+            raise ValueError("scale must be finite")
+        coef_ptr = 0 if coef is None else _one(coef, torch.float32, device, "coef")
+        (b1, b2), L, stream = self.betas, hip.lib(), hip._stream(self._table)
+        step_ptr = _one(step, torch.int64, device, "step") if isinstance(step, torch.Tensor) else 0
+        lr_ptr = _one(lr, torch.float32, device, "lr") if isinstance(lr, torch.Tensor) else 0
+        t = 1 if step_ptr else int(step)
+        rate = self.lr if lr is None or lr_ptr else float(lr)
+        if t < 1:
+            raise ValueError("step counts from 1")
+        if not 0 <= rate < math.inf:
+            raise ValueError("lr must not be negative")
+        key = (self.seed * 0x85EBCA6B + t * 0xC2B2AE35) & 0xFFFFFFFF
+        hyper = (b1, 1 - b1, b2, 1 - b2, self.eps, 1 - rate * self.weight_decay, rate / (1 - b1 ** t),
+                 1 / math.sqrt(1 - b2 ** t), scale, key ^ key >> 16)
+        on_device = 0
+        if step_ptr or lr_ptr:
+            numbers = torch.empty(L.netop_adamw_hyper_bytes(), dtype=torch.uint8, device=self.device)
+            on_device = numbers.data_ptr()
+            hip._check(L.netop_adamw_hyper(on_device, _HYPER.pack(*hyper), b1, b2, rate, self.weight_decay, self.seed,
+                                           lr_ptr, step_ptr, t, device, stream), "netop_adamw_hyper")
+        eight = self.state_bits == 8
+        at = ptrs.buffer_info()[0]
+        for a, b, chunks, n in self._launches:
+            if n == 0:
+                continue  # nothing but empty tensors
+            block = _STEP.pack(chunks, 0 if self.master is None else self.master.data_ptr(), self.exp_avg.data_ptr(),
+                               self.exp_avg_sq.data_ptr(), self.exp_avg_scale.data_ptr() if eight else 0,
+                               self.exp_avg_sq_scale.data_ptr() if eight else 0, coef_ptr, on_device, *hyper, n,
+                               self._kind, kinds[gtype], self.state_bits, b - a, device)
+            hip._check(L.netop_adamw_step(block, at + 8 * a, stream), "netop_adamw_step")

@@ -68,14 +68,22 @@ def lib() -> ctypes.CDLL:
             L.netop_shm_barrier_close.restype = None
             L.netop_shm_unlink.argtypes = [ctypes.c_char_p]
             L.netop_shm_unlink.restype = i32
-            # norm.hip: what follows a reduction (norm.py packs the parameter blocks)
-            block = ctypes.c_char_p
+            # norm.hip, adamw.hip: what follows a reduction (norm.py, adamw.py pack the parameter blocks)
+            block, f32, f64, i64 = ctypes.c_char_p, ctypes.c_float, ctypes.c_double, ctypes.c_int64
             L.netop_add_rms_norm.argtypes = [block, vp]
             L.netop_add_rms_norm.restype = i32
             L.netop_norm_backward_parts.argtypes = [u64, i32]
             L.netop_norm_backward_parts.restype = i32
             L.netop_add_rms_norm_backward.argtypes = [block, vp]
             L.netop_add_rms_norm_backward.restype = i32
+            for f in (L.netop_adamw_chunk, L.netop_adamw_max_grads, L.netop_adamw_hyper_bytes):
+                f.argtypes, f.restype = [], i32
+            L.netop_adamw_step.argtypes = [block, vp, vp]
+            L.netop_adamw_step.restype = i32
+            L.netop_adamw_hyper.argtypes = [vp, block, f64, f64, f64, f64, u32, vp, vp, i64, i32, vp]
+            L.netop_adamw_hyper.restype = i32
+            L.netop_grad_norm.argtypes = [vp, vp, i32, i32, u64, vp, u64, vp, vp, vp, f32, f32, i32, vp]
+            L.netop_grad_norm.restype = i32
             _lib = L
     return _lib
 

@@ -107,8 +107,11 @@ __device__ __forceinline__ void store4(T* p, const Vec<float, 4>& v, int n) {
         if (j < n) p[j] = T(v[j]);
 }
 
+// Products and sums are rounded one by one, not contracted: which way a state rounds hangs on the last
+// bit, and is to follow from the formulas alone, whatever compiled them.
 template <class P, class G, int BITS>
 __global__ __launch_bounds__(kThreads) void adamw_kernel(StepParams a, Grads grads) {
+#pragma clang fp contract(off)
     constexpr bool kMaster = sizeof(P) == 2;
     const Chunk ch = a.chunks[blockIdx.x];
     const G* gp = static_cast<const G*>(grads.at[ch.tensor]);
@@ -173,8 +176,10 @@ __global__ __launch_bounds__(kThreads) void adamw_kernel(StepParams a, Grads gra
         } else {
             m_max = lanes_max<64, false>(m_max);
             r_max = lanes_max<64, false>(r_max);
-            const float m_inv = m_max < kTiny ? 0.0f : kE4m3Max / m_max;
-            const float r_inv = r_max < kTiny ? 0.0f : kE4m3Max / r_max;
+            const float m_scale = m_max < kTiny ? 0.0f : m_max * (1.0f / kE4m3Max);
+            const float r_scale = r_max < kTiny ? 0.0f : r_max * (1.0f / kE4m3Max);
+            const float m_inv = m_max < kTiny ? 0.0f : 1.0f / m_scale;
+            const float r_inv = r_max < kTiny ? 0.0f : 1.0f / r_scale;
             uint32_t mw = 0, vw = 0;
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
@@ -191,8 +196,8 @@ __global__ __launch_bounds__(kThreads) void adamw_kernel(StepParams a, Grads gra
             __builtin_nontemporal_store(mw, reinterpret_cast<uint32_t*>(static_cast<char*>(a.m) + at));
             __builtin_nontemporal_store(vw, reinterpret_cast<uint32_t*>(static_cast<char*>(a.v) + at));
             if (lane == 0) {
-                a.m_scale[at / kBlock] = m_max < kTiny ? 0.0f : m_max / kE4m3Max;
-                a.v_scale[at / kBlock] = r_max < kTiny ? 0.0f : r_max / kE4m3Max;
+                a.m_scale[at / kBlock] = m_scale;
+                a.v_scale[at / kBlock] = r_scale;
             }
         }
     }

@@ -62,13 +62,13 @@ struct NormBackwardParams {
 };
 static_assert(sizeof(NormParams) == 240 && sizeof(NormBackwardParams) == 128, "ops/norm.py packs these");
 
-// The sum of x over the TPR threads of a row, in every one of them.  `red`: TPR / 64 floats that
+// The sum of x over the TPR threads of a row, in every one of them.  `red`: the row's TPR / 64 floats, which
 // the workgroup has not read since its last barrier.
 template <int TPR>
 __device__ __forceinline__ float row_sum(float x, float* red) {
-    x = lanes_sum<64>(x);
+    x = lanes_sum<(TPR < 64 ? TPR : 64)>(x);
     if constexpr (TPR > 64) {
-        if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = x;
+        if ((threadIdx.x & 63) == 0) red[threadIdx.x % TPR >> 6] = x;
         __syncthreads();
         x = 0;
 #pragma unroll
@@ -78,9 +78,9 @@ __device__ __forceinline__ float row_sum(float x, float* red) {
 }
 template <int TPR>
 __device__ __forceinline__ float row_max(float x, float* red) {
-    x = lanes_max<64, true>(x);
+    x = lanes_max<(TPR < 64 ? TPR : 64), true>(x);
     if constexpr (TPR > 64) {
-        if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = x;
+        if ((threadIdx.x & 63) == 0) red[threadIdx.x % TPR >> 6] = x;
         __syncthreads();
         x = red[0];
 #pragma unroll
@@ -89,237 +89,368 @@ __device__ __forceinline__ float row_max(float x, float* red) {
     return x;
 }
 
-template <class T>
-__device__ __forceinline__ Vec<float, 8> load8(const T* p, int n) {  // n < 8 elements, zeros behind
-    Vec<float, 8> v = 0.0f;
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
-        if (j < n) v[j] = float(p[j]);
-    return v;
-}
-
-template <class T>
-__device__ __forceinline__ Vec<float, 8> weights8(const void* w, int f32, int c, int n) {
-    if (f32) {
-        const float* p = static_cast<const float*>(w) + c;
-        return n >= 8 ? Wide<float, 8>::load(p) : load8(p, n);
+// Vectors of a row.  TPR threads hold it, VPT vectors of 8 columns each: vector k of thread t is columns
+// 8 (k TPR + t) and on.  One that would end behind the row is the row's last eight columns instead: every
+// load and store stays one instruction without a branch, columns that two threads hold come out the same
+// in both, and sums count them once (`twice` columns are left out).  Taking such a vector element by
+// element made a row of 5004 columns a third slower than one of 5008.  Rows have 8 columns at least.
+// WHOLE: the width is a multiple of eight, and none of this arises.
+template <bool WHOLE>
+struct At {
+    int c, twice;
+    bool in;
+    __device__ __forceinline__ At(int vec, int cols) : in(vec * 8 < cols) {
+        c = WHOLE || vec * 8 + 8 <= cols ? vec * 8 : cols - 8;
+        twice = WHOLE ? 0 : vec * 8 - c;
     }
-    const T* p = static_cast<const T*>(w) + c;
-    return n >= 8 ? widen<T, 8>(Wide<T, 8>::load(p)) : load8(p, n);
+};
+
+template <class T, int TPR, int VPT, bool WHOLE, bool STREAM>
+struct Row {
+    Vec<T, 8> v[VPT];
+    __device__ __forceinline__ void load(const T* p, int t, int cols) {
+#pragma unroll
+        for (int k = 0; k < VPT; ++k) {
+            const At<WHOLE> at(k * TPR + t, cols);
+            if (at.in) v[k] = STREAM ? Wide<T, 8>::stream(p + at.c) : Wide<T, 8>::load(p + at.c);
+        }
+    }
+};
+
+__device__ __forceinline__ float dot8(const Vec<float, 8>& x, const Vec<float, 8>& y, int twice, float s) {
+    if (twice) {
+#pragma unroll
+        for (int j = 1; j < 8; ++j) s = fmaf(j >= twice ? x[j] : 0.0f, y[j], s);
+        return s;
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) s = fmaf(x[j], y[j], s);
+    return s;
 }
 
 template <class T>
-__device__ __forceinline__ void store8(T* p, const Vec<float, 8>& v, int n) {
-    if (n >= 8) {
-        Wide<T, 8>::store(p, narrow<T, 8>(v));
-        return;
-    }
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
-        if (j < n) p[j] = T(v[j]);
+__device__ __forceinline__ Vec<float, 8> weights8(const void* w, int f32, int c) {
+    return f32 ? Wide<float, 8>::load(static_cast<const float*>(w) + c)
+               : widen<T, 8>(Wide<T, 8>::load(static_cast<const T*>(w) + c));
 }
 
-// TPR threads hold a row, VPT vectors of 8 columns each: vector k of thread t is columns
-// 8 (k TPR + t) and on.
-template <class T, int TPR, int VPT, int OUT>
+// The larger of two magnitudes; NaN stays.
+__device__ __forceinline__ float larger(float x, float y) { return x > y || x != x ? x : y; }
+
+// AHEAD inputs are on their way together: with peer pointers each is an xGMI round trip.
+template <class T, int TPR, int VPT, int AHEAD, bool E4M3, bool WHOLE, bool STREAM>
 __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void norm_kernel(NormParams a) {
     constexpr int kRows = TPR < 256 ? 256 / TPR : 1;
-    __shared__ float red[2][TPR / 64];
+    __shared__ float red[2][TPR < 64 ? 1 : TPR / 64 * kRows];
     const uint64_t row = uint64_t(blockIdx.x) * kRows + threadIdx.x / TPR;
-    if (kRows > 1 && row >= a.rows) return;  // whole wavefronts: such rows meet no barrier
+    const bool here = row < a.rows;
+    if (TPR <= 64 && !here) return;  // all threads of a row, and rows of a wavefront or less meet no barrier
     const int t = threadIdx.x % TPR;
-    const int cols = a.cols;
+    const int cols = here ? a.cols : 0;
     Vec<float, 8> h[VPT];
 #pragma unroll
     for (int k = 0; k < VPT; ++k) h[k] = 0.0f;
-    // Loads of kAhead inputs are in flight together: with peer pointers each is an xGMI round trip.
-    constexpr int kAhead = 8 / VPT > 0 ? 8 / VPT : 1;
-    for (int s0 = 0; s0 < a.n_in; s0 += kAhead) {
-        Vec<T, 8> v[kAhead][VPT];
+    for (int s0 = 0; s0 < a.n_in; s0 += AHEAD) {
+        Row<T, TPR, VPT, WHOLE, STREAM> in[AHEAD];
 #pragma unroll
-        for (int s = 0; s < kAhead; ++s) {
-            if (s0 + s >= a.n_in) break;
-            const T* p = static_cast<const T*>(a.in[s0 + s]) + int64_t(row) * a.in_stride[s0 + s];
+        for (int s = 0; s < AHEAD; ++s)
+            if (s0 + s < a.n_in) in[s].load(static_cast<const T*>(a.in[s0 + s]) + int64_t(row) * a.in_stride[s0 + s], t, cols);
 #pragma unroll
-            for (int k = 0; k < VPT; ++k) {
-                const int c = (k * TPR + t) * 8;
-                if (c + 8 <= cols) v[s][k] = Wide<T, 8>::load(p + c);
+        for (int s = 0; s < AHEAD; ++s)
+            if (s0 + s < a.n_in) {
+#pragma unroll
+                for (int k = 0; k < VPT; ++k)
+                    if (At<WHOLE>(k * TPR + t, cols).in) h[k] += widen<T, 8>(in[s].v[k]);
             }
-        }
-#pragma unroll
-        for (int s = 0; s < kAhead; ++s) {
-            if (s0 + s >= a.n_in) break;
-#pragma unroll
-            for (int k = 0; k < VPT; ++k) {
-                const int c = (k * TPR + t) * 8;
-                if (c + 8 <= cols) {
-                    h[k] += widen<T, 8>(v[s][k]);
-                } else if (c < cols) {
-                    const T* p = static_cast<const T*>(a.in[s0 + s]) + int64_t(row) * a.in_stride[s0 + s];
-                    h[k] += load8(p + c, cols - c);
-                }
-            }
-        }
     }
     float ss = 0;
 #pragma unroll
-    for (int k = 0; k < VPT; ++k)
-#pragma unroll
-        for (int j = 0; j < 8; ++j) ss = fmaf(h[k][j], h[k][j], ss);
-    ss = row_sum<TPR>(ss, red[0]);
-    const float rstd = 1.0f / sqrtf(ss / float(cols) + a.eps);
-    if (a.rstd && t == 0) a.rstd[row] = rstd;
+    for (int k = 0; k < VPT; ++k) {
+        const At<WHOLE> at(k * TPR + t, cols);
+        if (at.in) ss = dot8(h[k], h[k], at.twice, ss);
+    }
+    const int slot = TPR < 64 ? 0 : int(threadIdx.x) / TPR * (TPR / 64);
+    ss = row_sum<TPR>(ss, red[0] + slot);
+    const float rstd = 1.0f / sqrtf(ss / float(a.cols) + a.eps);
+    if (a.rstd && t == 0 && here) a.rstd[row] = rstd;
     if (a.h) {  // after the reduction: every thread of the row has read its inputs, which h may replace
         T* p = static_cast<T*>(a.h) + int64_t(row) * a.h_stride;
 #pragma unroll
         for (int k = 0; k < VPT; ++k) {
-            const int c = (k * TPR + t) * 8;
-            if (c < cols) store8(p + c, h[k], cols - c);
+            const At<WHOLE> at(k * TPR + t, cols);
+            if (at.in) Wide<T, 8>::store(p + at.c, narrow<T, 8>(h[k]));
         }
     }
     float amax = 0;
 #pragma unroll
     for (int k = 0; k < VPT; ++k) {
-        const int c = (k * TPR + t) * 8;
-        if (c < cols) h[k] = h[k] * rstd * weights8<T>(a.weight, a.weight_f32, c, cols - c);
-        if constexpr (OUT == kRowScale) {
+        const At<WHOLE> at(k * TPR + t, cols);
+        if (at.in) h[k] = h[k] * rstd * weights8<T>(a.weight, a.weight_f32, at.c);
+        if constexpr (E4M3) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const float y = fabsf(h[k][j]);
-                amax = amax > y || amax != amax ? amax : y;
-            }
+            for (int j = 0; j < 8; ++j) amax = larger(amax, fabsf(h[k][j]));
         }
     }
-    if constexpr (OUT == kSame) {
+    if constexpr (!E4M3) {
         T* p = static_cast<T*>(a.out) + int64_t(row) * a.out_stride;
 #pragma unroll
         for (int k = 0; k < VPT; ++k) {
-            const int c = (k * TPR + t) * 8;
-            if (c < cols) store8(p + c, h[k], cols - c);
+            const At<WHOLE> at(k * TPR + t, cols);
+            if (at.in) Wide<T, 8>::store(p + at.c, narrow<T, 8>(h[k]));
         }
     } else {
         uint8_t* p = static_cast<uint8_t*>(a.out) + int64_t(row) * a.out_stride;
-        if constexpr (OUT == kRowScale) {
-            amax = row_max<TPR>(amax, red[1]);
-            if (t == 0) a.scales[row] = amax < kTiny ? 0.0f : amax / kE4m3Max;
-        }
+        const bool by_group = a.out_kind == kGroupScale;
         const int groups = (cols + kGroup - 1) / kGroup;
+        if (!by_group) {
+            amax = row_max<TPR>(amax, red[1] + slot);
+            if (t == 0 && here) a.scales[row] = amax < kTiny ? 0.0f : amax / kE4m3Max;
+        }
 #pragma unroll
         for (int k = 0; k < VPT; ++k) {
-            const int c = (k * TPR + t) * 8;
-            if constexpr (OUT == kGroupScale) {  // 16 neighbouring threads hold a group
+            const At<WHOLE> at(k * TPR + t, cols);
+            if (by_group) {  // 16 neighbouring threads hold a group
                 amax = 0;
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const float y = fabsf(h[k][j]);
-                    amax = amax > y || amax != amax ? amax : y;
-                }
-                amax = lanes_max<16, true>(amax);
-                if ((t & 15) == 0 && c < cols) a.scales[row * groups + c / kGroup] = amax < kTiny ? 0.0f : amax / kE4m3Max;
+                for (int j = 0; j < 8; ++j) amax = j >= at.twice ? larger(amax, fabsf(h[k][j])) : amax;
+                amax = lanes_max<(TPR < 16 ? TPR : 16), true>(amax);
+                if ((t & 15) == 0 && at.in) a.scales[row * groups + (k * TPR + t) / 16] = amax < kTiny ? 0.0f : amax / kE4m3Max;
             }
             const float inv = amax < kTiny ? 0.0f : kE4m3Max / amax;
-            if (c < cols) {
-                Vec<float, 8> q;
+            if (!at.in) continue;
+            Vec<float, 8> q;
 #pragma unroll
-                for (int j = 0; j < 8; ++j) q[j] = clamp_e4m3(h[k][j] * inv);
-                Vec<uint32_t, 2> w;
-                w[0] = pack_e4m3(q[0], q[1], q[2], q[3]);
-                w[1] = pack_e4m3(q[4], q[5], q[6], q[7]);
-                if (cols - c >= 8) {
-                    const auto bytes = __builtin_bit_cast(decltype(Vec<uint8_t, 8>()), w);
-                    Wide<uint8_t, 8>::store(p + c, bytes);
-                } else {
+            for (int j = 0; j < 8; ++j) q[j] = clamp_e4m3(h[k][j] * inv);
+            Vec<uint32_t, 2> w;
+            w[0] = pack_e4m3(q[0], q[1], q[2], q[3]);
+            w[1] = pack_e4m3(q[4], q[5], q[6], q[7]);
+            if (by_group && at.twice) {  // its first columns may be of the group before, with another scale
 #pragma unroll
-                    for (int j = 0; j < 7; ++j)
-                        if (j < cols - c) p[c + j] = uint8_t(w[j >> 2] >> (8 * (j & 3)));
-                }
+                for (int j = 1; j < 8; ++j)
+                    if (j >= at.twice) p[at.c + j] = uint8_t(w[j >> 2] >> (8 * (j & 3)));
+            } else {
+                const auto bytes = __builtin_bit_cast(decltype(Vec<uint8_t, 8>()), w);
+                Wide<uint8_t, 8>::store(p + at.c, bytes);
             }
         }
     }
+}
+
+// Rows of less than eight columns: a thread each.
+template <class T>
+__global__ __launch_bounds__(256) void narrow_norm_kernel(NormParams a) {
+    const uint64_t row = uint64_t(blockIdx.x) * 256 + threadIdx.x;
+    if (row >= a.rows) return;
+    float h[7], y[7], ss = 0, amax = 0;
+#pragma unroll
+    for (int c = 0; c < 7; ++c) h[c] = y[c] = 0;
+    for (int s = 0; s < a.n_in; ++s) {
+        const T* p = static_cast<const T*>(a.in[s]) + int64_t(row) * a.in_stride[s];
+#pragma unroll
+        for (int c = 0; c < 7; ++c)
+            if (c < a.cols) h[c] += float(p[c]);
+    }
+#pragma unroll
+    for (int c = 0; c < 7; ++c) ss = fmaf(h[c], h[c], ss);
+    const float rstd = 1.0f / sqrtf(ss / float(a.cols) + a.eps);
+    if (a.rstd) a.rstd[row] = rstd;
+#pragma unroll
+    for (int c = 0; c < 7; ++c)
+        if (c < a.cols) {
+            if (a.h) (static_cast<T*>(a.h) + int64_t(row) * a.h_stride)[c] = T(h[c]);
+            y[c] = h[c] * rstd * (a.weight_f32 ? static_cast<const float*>(a.weight)[c] : float(static_cast<const T*>(a.weight)[c]));
+            amax = larger(amax, fabsf(y[c]));
+        }
+    const float inv = amax < kTiny ? 0.0f : kE4m3Max / amax;
+    if (a.out_kind != kSame) a.scales[row] = amax < kTiny ? 0.0f : amax / kE4m3Max;
+#pragma unroll
+    for (int c = 0; c < 7; ++c)
+        if (c < a.cols) {
+            if (a.out_kind == kSame)
+                (static_cast<T*>(a.out) + int64_t(row) * a.out_stride)[c] = T(y[c]);
+            else
+                (static_cast<uint8_t*>(a.out) + int64_t(row) * a.out_stride)[c] =
+                    uint8_t(pack_e4m3(clamp_e4m3(y[c] * inv), 0, 0, 0));
+        }
 }
 
 // Each row's share of dweight stays in the registers of the thread that holds those columns; a
-// workgroup walks rows in steps of the grid and writes one partial row in the end, which
-// dweight_kernel adds up in a fixed order: no atomics, the same bits every time.
-template <class T, int TPR, int VPT>
+// workgroup walks rows in steps of the grid, adds up its rows' shares and writes one partial row,
+// and dweight_kernel adds those up: a fixed order, no atomics, the same bits every time.  With four
+// vectors a thread 128 registers do not hold a row beside dweight, and it is read a second time, out of
+// the caches.  (Fetching the next row ahead costs as many registers and gained nothing: 53 against 51 us
+// at 8192 x 4096.)
+template <class T, int TPR, int VPT, bool WHOLE, bool STREAM>
 __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void norm_backward_kernel(NormBackwardParams a) {
     constexpr int kRows = TPR < 256 ? 256 / TPR : 1;
-    __shared__ float red[2][TPR / 64];
-    const int part = int(blockIdx.x) * kRows + int(threadIdx.x) / TPR;
-    if (kRows > 1 && part >= a.parts) return;  // whole wavefronts, as above
-    const int t = threadIdx.x % TPR;
-    const int cols = a.cols;
-    Vec<float, 8> dw[VPT];
+    constexpr bool kTwice = VPT == 4;
+    __shared__ float red[2][TPR < 64 ? 1 : TPR / 64 * kRows];
+    const int t = threadIdx.x % TPR, r = int(threadIdx.x) / TPR;
+    const int slot = TPR < 64 ? 0 : r * (TPR / 64);
+    const uint64_t first = uint64_t(blockIdx.x) * kRows, walk = uint64_t(gridDim.x) * kRows;
+    Vec<float, 8> dw[VPT], weight[VPT];
 #pragma unroll
-    for (int k = 0; k < VPT; ++k) dw[k] = 0.0f;
+    for (int k = 0; k < VPT; ++k) {
+        dw[k] = 0.0f;
+        const At<WHOLE> at(k * TPR + t, a.cols);
+        if (!kTwice && at.in) weight[k] = weights8<T>(a.weight, a.weight_f32, at.c);
+    }
     int turn = 0;
-    for (uint64_t row = part; row < a.rows; row += a.parts, turn ^= 1) {
+    // Rows that share barriers take as many turns as the workgroup's first.
+    for (uint64_t base = first, row = first + r; (TPR <= 64 ? row : base) < a.rows; base += walk, row += walk, turn ^= 1) {
+        const int cols = row < a.rows ? a.cols : 0;
+        const float rstd = cols ? a.rstd[row] : 0.0f;
         const T* dy = static_cast<const T*>(a.dy) + int64_t(row) * a.dy_stride;
         const T* hp = static_cast<const T*>(a.h) + int64_t(row) * a.h_stride;
-        const float rstd = a.rstd[row];
-        Vec<float, 8> g[VPT], h[VPT];
+        const T* rp = a.dres ? static_cast<const T*>(a.dres) + int64_t(row) * a.dres_stride : nullptr;
+        T* dh = static_cast<T*>(a.dh) + int64_t(row) * a.dh_stride;
+        Row<T, TPR, VPT, WHOLE, STREAM> raw_g, raw_h, raw_r;
+        if constexpr (!kTwice) {
+            raw_g.load(dy, t, cols);
+            raw_h.load(hp, t, cols);
+            if (rp) raw_r.load(rp, t, cols);
+        }
+        Vec<float, 8> g[VPT];
         float dot = 0;
 #pragma unroll
         for (int k = 0; k < VPT; ++k) {
-            const int c = (k * TPR + t) * 8;
-            g[k] = h[k] = 0.0f;
-            if (c + 8 <= cols) {
-                g[k] = widen<T, 8>(Wide<T, 8>::load(dy + c));
-                h[k] = widen<T, 8>(Wide<T, 8>::load(hp + c));
-            } else if (c < cols) {
-                g[k] = load8(dy + c, cols - c);
-                h[k] = load8(hp + c, cols - c);
+            const At<WHOLE> at(k * TPR + t, cols);
+            if (at.in) {
+                if constexpr (kTwice) {
+                    raw_g.v[k] = Wide<T, 8>::load(dy + at.c);
+                    raw_h.v[k] = Wide<T, 8>::load(hp + at.c);
+                }
+                g[k] = widen<T, 8>(raw_g.v[k]);
+                const Vec<float, 8> h = widen<T, 8>(raw_h.v[k]);
+                dw[k] += g[k] * h * rstd;
+                if constexpr (kTwice) weight[k] = weights8<T>(a.weight, a.weight_f32, at.c);
+                g[k] *= weight[k];
+                dot = dot8(g[k], h, at.twice, dot);
             }
+            if constexpr (kTwice) asm volatile("" ::: "memory");  // holds back the next vector's loads
         }
+        dot = row_sum<TPR>(dot, red[turn] + slot);
+        const float back = rstd * rstd * rstd * (dot / float(a.cols));
 #pragma unroll
         for (int k = 0; k < VPT; ++k) {
-            const int c = (k * TPR + t) * 8;
-            dw[k] += g[k] * h[k] * rstd;
-            if (c < cols) g[k] *= weights8<T>(a.weight, a.weight_f32, c, cols - c);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) dot = fmaf(g[k][j], h[k][j], dot);
+            const At<WHOLE> at(k * TPR + t, cols);
+            if (at.in) {
+                if constexpr (kTwice) {
+                    g[k] = widen<T, 8>(Wide<T, 8>::load(dy + at.c)) * weights8<T>(a.weight, a.weight_f32, at.c);
+                    raw_h.v[k] = Wide<T, 8>::load(hp + at.c);
+                    if (rp) raw_r.v[k] = Wide<T, 8>::load(rp + at.c);
+                }
+                g[k] = rstd * g[k] - widen<T, 8>(raw_h.v[k]) * back;
+                if (rp) g[k] += widen<T, 8>(raw_r.v[k]);
+            }
+            if constexpr (kTwice) asm volatile("" ::: "memory");
         }
-        dot = row_sum<TPR>(dot, red[turn]);
-        const float back = rstd * rstd * rstd * (dot / float(cols));
-        T* dh = static_cast<T*>(a.dh) + int64_t(row) * a.dh_stride;
-        const T* dres = static_cast<const T*>(a.dres) + (a.dres ? int64_t(row) * a.dres_stride : 0);
+        if constexpr (kTwice) __syncthreads();  // dh may be where two threads have just read the same columns
 #pragma unroll
         for (int k = 0; k < VPT; ++k) {
-            const int c = (k * TPR + t) * 8;
-            if (c >= cols) continue;
-            Vec<float, 8> d = rstd * g[k] - h[k] * back;
-            if (a.dres) d += cols - c >= 8 ? widen<T, 8>(Wide<T, 8>::load(dres + c)) : load8(dres + c, cols - c);
-            store8(dh + c, d, cols - c);
+            const At<WHOLE> at(k * TPR + t, cols);
+            if (at.in) Wide<T, 8>::store(dh + at.c, narrow<T, 8>(g[k]));
         }
+    }
+    if constexpr (kRows > 1) {
+        __shared__ Vec<float, 8> shares[kRows][TPR];
+        shares[r][t] = dw[0];
+        __syncthreads();
+        if (r) return;
+#pragma unroll
+        for (int i = 1; i < kRows; ++i) dw[0] += shares[i][t];
     }
 #pragma unroll
     for (int k = 0; k < VPT; ++k) {
-        const int c = (k * TPR + t) * 8;
-        if (c < cols) store8(a.partial + uint64_t(part) * cols + c, dw[k], cols - c);
+        const At<WHOLE> at(k * TPR + t, a.cols);
+        if (at.in) Wide<float, 8>::store(a.partial + uint64_t(blockIdx.x) * a.cols + at.c, dw[k]);
     }
 }
 
-// dweight[c] = sum of partial[.][c]: 32 columns x 32 strands of parts a workgroup.
+template <class T>
+__global__ __launch_bounds__(256) void narrow_backward_kernel(NormBackwardParams a) {
+    __shared__ float shares[4][7];
+    float dw[7], w[7];
+#pragma unroll
+    for (int c = 0; c < 7; ++c) {
+        dw[c] = w[c] = 0;
+        if (c < a.cols) w[c] = a.weight_f32 ? static_cast<const float*>(a.weight)[c] : float(static_cast<const T*>(a.weight)[c]);
+    }
+    for (uint64_t row = uint64_t(blockIdx.x) * 256 + threadIdx.x; row < a.rows; row += uint64_t(gridDim.x) * 256) {
+        const T* dy = static_cast<const T*>(a.dy) + int64_t(row) * a.dy_stride;
+        const T* hp = static_cast<const T*>(a.h) + int64_t(row) * a.h_stride;
+        const T* rp = a.dres ? static_cast<const T*>(a.dres) + int64_t(row) * a.dres_stride : nullptr;
+        T* dh = static_cast<T*>(a.dh) + int64_t(row) * a.dh_stride;
+        const float rstd = a.rstd[row];
+        float g[7], h[7], dot = 0;
+#pragma unroll
+        for (int c = 0; c < 7; ++c) {
+            g[c] = h[c] = 0;
+            if (c < a.cols) {
+                g[c] = float(dy[c]);
+                h[c] = float(hp[c]);
+            }
+            dw[c] += g[c] * h[c] * rstd;
+            g[c] *= w[c];
+            dot = fmaf(g[c], h[c], dot);
+        }
+        const float back = rstd * rstd * rstd * (dot / float(a.cols));
+#pragma unroll
+        for (int c = 0; c < 7; ++c)
+            if (c < a.cols) dh[c] = T(rstd * g[c] - h[c] * back + (rp ? float(rp[c]) : 0.0f));
+    }
+#pragma unroll
+    for (int c = 0; c < 7; ++c) {
+        dw[c] = lanes_sum<64>(dw[c]);
+        if ((threadIdx.x & 63) == 0) shares[threadIdx.x >> 6][c] = dw[c];
+    }
+    __syncthreads();
+    const int c = threadIdx.x;
+    if (c < a.cols)
+        a.partial[uint64_t(blockIdx.x) * a.cols + c] = shares[0][c] + shares[1][c] + shares[2][c] + shares[3][c];
+}
+
+// dweight[c] = sum of partial[.][c]: 64 columns (16 lanes x 4) and 64 strands of parts a workgroup.
 __global__ __launch_bounds__(1024) void dweight_kernel(const float* __restrict__ partial, int parts, int cols,
                                                        void* __restrict__ dweight, int dtype) {
-    __shared__ float sum[32][33];
-    const int x = threadIdx.x & 31, y = threadIdx.x >> 5;
-    const int c = blockIdx.x * 32 + x;
-    float s = 0;
-    if (c < cols)
-        for (int p = y; p < parts; p += 32) s += partial[uint64_t(p) * cols + c];
-    sum[y][x] = s;
-    __syncthreads();
-    if (y == 0 && c < cols) {
-        s = 0;
+    __shared__ float sum[16][64];
+    const int x = threadIdx.x & 15, y = threadIdx.x >> 4;
+    const int c = blockIdx.x * 64 + x * 4;
+    Vec<float, 4> s = 0.0f;
+    if (c + 4 <= cols) {
+        int p = y;
+        for (; p + 192 < parts; p += 256) {  // four loads in flight
+            Vec<float, 4> v[4];
 #pragma unroll
-        for (int i = 0; i < 32; ++i) s += sum[i][x];
+            for (int u = 0; u < 4; ++u) v[u] = Wide<float, 4>::load(partial + uint64_t(p + 64 * u) * cols + c);
+#pragma unroll
+            for (int u = 0; u < 4; ++u) s += v[u];
+        }
+        for (; p < parts; p += 64) s += Wide<float, 4>::load(partial + uint64_t(p) * cols + c);
+    } else if (c < cols) {
+        for (int p = y; p < parts; p += 64)
+#pragma unroll
+            for (int j = 0; j < 3; ++j)
+                if (c + j < cols) s[j] += partial[uint64_t(p) * cols + c + j];
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {  // the four strands of a wavefront, then the sixteen wavefronts
+        s[j] += __shfl_xor(s[j], 16, 64);
+        s[j] += __shfl_xor(s[j], 32, 64);
+        if ((threadIdx.x & 48) == 0) sum[threadIdx.x >> 6][x * 4 + j] = s[j];
+    }
+    __syncthreads();
+    const int i = threadIdx.x, at = blockIdx.x * 64 + i;
+    if (i < 64 && at < cols) {
+        float all = 0;
+#pragma unroll
+        for (int w = 0; w < 16; ++w) all += sum[w][i];
         if (dtype == kF32)
-            static_cast<float*>(dweight)[c] = s;
+            static_cast<float*>(dweight)[at] = all;
         else if (dtype == kBf16)
-            static_cast<__bf16*>(dweight)[c] = __bf16(s);
+            static_cast<__bf16*>(dweight)[at] = __bf16(all);
         else
-            static_cast<_Float16*>(dweight)[c] = _Float16(s);
+            static_cast<_Float16*>(dweight)[at] = _Float16(all);
     }
 }
 
@@ -328,57 +459,95 @@ struct Shape {
     int tpr, vpt;
 };
 
-Shape shape_for(int cols) {
+// One vector a thread up to 4096 columns: fewest registers, most rows in flight.  Beyond, a row of two
+// vectors a thread leaves each CU two workgroups (16384 x 8192 bf16 to e4m3: 176 us with 512 threads, 202 with
+// 1024), while few rows end sooner spread wider (64 x 8192, 8 partial sums: 5.3 us with 1024, 6.6 with 512).
+Shape shape_for(int cols, uint64_t rows) {
     const int vecs = (cols + 7) / 8;
-    if (vecs <= 64) return {64, 1};
-    if (vecs <= 128) return {64, 2};
-    if (vecs <= 256) return {256, 1};
-    if (vecs <= 512) return {256, 2};
-    if (vecs <= 1024) return {256, 4};
-    if (vecs <= 2048) return {1024, 2};
-    return {1024, 4};
+    for (int tpr = 8; tpr <= 512; tpr *= 2)
+        if (vecs <= tpr) return {tpr, 1};
+    if (vecs <= 1024) return rows > 1024 ? Shape{512, 2} : Shape{1024, 1};
+    return vecs <= 2048 ? Shape{1024, 2} : Shape{1024, 4};
+}
+
+// Workgroups of the backward pass, each with a partial row of dweight: enough to fill the chip, few enough
+// that their rows cost little next to the data.
+int parts_for(int cols, uint64_t rows) {
+    const int tpr = cols < 8 ? 1 : shape_for(cols, rows).tpr;
+    const uint64_t at_once = tpr < 256 ? 256 / tpr : 1;
+    const uint64_t most = tpr < 256 ? 1024 : rows >= 2048 ? 512 : 256, need = (rows + at_once - 1) / at_once;
+    return int(need < most ? need : most);
+}
+
+// Inputs of 64 MiB and more are read past the caches: they hardly lie there (256 MB) and will not be read
+// again.  4096 x 4096 bf16 28.1 -> 25.7 us, backward 8192 x 4096 54 -> 51; inputs that do lie there are slower
+// that way (1001 x 5003, 3 partial sums: 15.0 -> 17.7).  Not fp32, whose vectors are two loads of half lines.
+bool past_caches(uint64_t rows, int cols, int inputs) {
+    return rows * uint64_t(cols) * uint64_t(inputs) * 2 >= 64u << 20;
 }
 
 template <class T, int TPR, int VPT>
 void launch_norm(const NormParams& a, hipStream_t stream) {
-    constexpr int kRows = TPR < 256 ? 256 / TPR : 1;
+    constexpr int kRows = TPR < 256 ? 256 / TPR : 1, kMany = 8 / VPT > 2 ? 8 / VPT : 2;
     const dim3 grid(unsigned((a.rows + kRows - 1) / kRows)), block(TPR < 256 ? 256 : TPR);
-    if (a.out_kind == kSame)
-        hipLaunchKernelGGL((norm_kernel<T, TPR, VPT, kSame>), grid, block, 0, stream, a);
-    else if (a.out_kind == kRowScale)
-        hipLaunchKernelGGL((norm_kernel<T, TPR, VPT, kRowScale>), grid, block, 0, stream, a);
-    else
-        hipLaunchKernelGGL((norm_kernel<T, TPR, VPT, kGroupScale>), grid, block, 0, stream, a);
+    const bool few = a.n_in <= 2, whole = a.cols % 8 == 0, eight = a.out_kind != kSame;
+    constexpr bool kStreams = sizeof(T) == 2;
+    const bool streams = kStreams && past_caches(a.rows, a.cols, a.n_in);
+    const auto k = !whole    ? eight ? norm_kernel<T, TPR, VPT, 2, true, false, false> : norm_kernel<T, TPR, VPT, 2, false, false, false>
+                   : !few    ? eight ? norm_kernel<T, TPR, VPT, kMany, true, true, false> : norm_kernel<T, TPR, VPT, kMany, false, true, false>
+                   : streams ? eight ? norm_kernel<T, TPR, VPT, 2, true, true, kStreams> : norm_kernel<T, TPR, VPT, 2, false, true, kStreams>
+                   : eight   ? norm_kernel<T, TPR, VPT, 2, true, true, false>
+                             : norm_kernel<T, TPR, VPT, 2, false, true, false>;
+    hipLaunchKernelGGL(k, grid, block, 0, stream, a);
 }
 
 template <class T, int TPR, int VPT>
 void launch_backward(const NormBackwardParams& a, hipStream_t stream) {
-    constexpr int kRows = TPR < 256 ? 256 / TPR : 1;
-    hipLaunchKernelGGL((norm_backward_kernel<T, TPR, VPT>), dim3(unsigned((a.parts + kRows - 1) / kRows)),
-                       dim3(TPR < 256 ? 256 : TPR), 0, stream, a);
+    constexpr bool kStreams = sizeof(T) == 2;
+    const auto k = a.cols % 8 ? norm_backward_kernel<T, TPR, VPT, false, false>
+                   : kStreams && past_caches(a.rows, a.cols, a.dres ? 3 : 2) ? norm_backward_kernel<T, TPR, VPT, true, kStreams>
+                                                                            : norm_backward_kernel<T, TPR, VPT, true, false>;
+    hipLaunchKernelGGL(k, dim3(unsigned(a.parts)), dim3(TPR < 256 ? 256 : TPR), 0, stream, a);
 }
 
-#define NETOP_FOR_SHAPE(s, CALL)                         \
-    do {                                                 \
-        if (s.tpr == 64 && s.vpt == 1) CALL(64, 1);      \
-        else if (s.tpr == 64) CALL(64, 2);               \
-        else if (s.tpr == 256 && s.vpt == 1) CALL(256, 1); \
-        else if (s.tpr == 256 && s.vpt == 2) CALL(256, 2); \
-        else if (s.tpr == 256) CALL(256, 4);             \
-        else if (s.vpt == 2) CALL(1024, 2);              \
-        else CALL(1024, 4);                              \
+#define NETOP_FOR_SHAPE(s, CALL)                    \
+    do {                                            \
+        switch (s.tpr) {                            \
+            case 8: CALL(8, 1); break;              \
+            case 16: CALL(16, 1); break;            \
+            case 32: CALL(32, 1); break;            \
+            case 64: CALL(64, 1); break;            \
+            case 128: CALL(128, 1); break;          \
+            case 256: CALL(256, 1); break;          \
+            case 512:                               \
+                if (s.vpt == 1) CALL(512, 1);       \
+                else CALL(512, 2);                  \
+                break;                              \
+            default:                                \
+                if (s.vpt == 1) CALL(1024, 1);      \
+                else if (s.vpt == 2) CALL(1024, 2); \
+                else CALL(1024, 4);                 \
+        }                                           \
     } while (0)
 
 template <class T>
 void norm_of(const NormParams& a, hipStream_t stream) {
-    const Shape s = shape_for(a.cols);
+    if (a.cols < 8) {
+        hipLaunchKernelGGL(narrow_norm_kernel<T>, dim3(unsigned((a.rows + 255) / 256)), dim3(256), 0, stream, a);
+        return;
+    }
+    const Shape s = shape_for(a.cols, a.rows);
 #define CALL(TPR, VPT) launch_norm<T, TPR, VPT>(a, stream)
     NETOP_FOR_SHAPE(s, CALL);
 #undef CALL
 }
 template <class T>
 void backward_of(const NormBackwardParams& a, hipStream_t stream) {
-    const Shape s = shape_for(a.cols);
+    if (a.cols < 8) {
+        hipLaunchKernelGGL(narrow_backward_kernel<T>, dim3(unsigned(a.parts)), dim3(256), 0, stream, a);
+        return;
+    }
+    const Shape s = shape_for(a.cols, a.rows);
 #define CALL(TPR, VPT) launch_backward<T, TPR, VPT>(a, stream)
     NETOP_FOR_SHAPE(s, CALL);
 #undef CALL
@@ -455,8 +624,7 @@ int netop_add_rms_norm(const NormParams* p, hipStream_t stream) {
 // How many rows of `cols` floats the backward pass needs as workspace.
 int netop_norm_backward_parts(uint64_t rows, int cols) {
     if (cols < 1 || cols > kMaxCols) return 0;
-    const uint64_t most = shape_for(cols).tpr == 64 ? 4096 : 1024;
-    return int(rows < most ? rows : most);
+    return parts_for(cols, rows);
 }
 
 int netop_add_rms_norm_backward(const NormBackwardParams* p, hipStream_t stream) {
@@ -485,7 +653,7 @@ int netop_add_rms_norm_backward(const NormBackwardParams* p, hipStream_t stream)
         const hipError_t e = hipGetLastError();
         if (e != hipSuccess) return int(e);
     }
-    hipLaunchKernelGGL(dweight_kernel, dim3(unsigned(p->cols + 31) / 32), dim3(1024), 0, stream, p->partial, p->parts,
+    hipLaunchKernelGGL(dweight_kernel, dim3(unsigned(p->cols + 63) / 64), dim3(1024), 0, stream, p->partial, p->parts,
                        p->cols, p->dweight, p->dweight_f32 ? int(kF32) : p->dtype);
     return int(hipGetLastError());
 }

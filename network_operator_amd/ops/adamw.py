@@ -30,10 +30,16 @@ _HYPER = struct.Struct("=9fI")
 _STEP = struct.Struct("=8Q" + "9fI" + "6i")
 
 
-def _dtypes():
+def _kinds():
+    """Type codes, once torch is there (the package is imported without it too)."""
+    global _KINDS
     import torch
 
-    return {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+    _KINDS = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+    return _KINDS
+
+
+_KINDS = None
 
 
 def _one(t, dtype, device, what):
@@ -58,7 +64,7 @@ def grad_norm(grads, total, *, norms=None, coef=None, max_norm=None, scale=1.0) 
     """
     import torch
 
-    kinds = _dtypes()
+    kinds = _KINDS or _kinds()
     first = next((g for g in grads if g is not None), None)
     if first is None:
         raise ValueError("no gradients")
@@ -70,13 +76,13 @@ def grad_norm(grads, total, *, norms=None, coef=None, max_norm=None, scale=1.0) 
         raise ValueError("max_norm must not be negative")
     if not math.isfinite(scale):
         raise ValueError("scale must be finite")
-    ptrs, ns = array("Q"), array("Q")
+    ptrs, ns = [], []
     for g in grads:
         if g is None:
             ptrs.append(0)
             ns.append(0)
             continue
-        if g.dtype != dtype:
+        if g.dtype is not dtype:
             raise ValueError(f"gradients must have one type: {dtype} and {g.dtype}")
         if not g.is_contiguous():
             raise ValueError("gradients must be contiguous")
@@ -101,9 +107,11 @@ def grad_norm(grads, total, *, norms=None, coef=None, max_norm=None, scale=1.0) 
         stretch *= 2
     stretches = elements // stretch + len(ns)
     work = torch.empty(stretches + len(ns), dtype=torch.float64, device=first.device)
-    hip._check(hip.lib().netop_grad_norm(ptrs.buffer_info()[0], ns.buffer_info()[0], len(ns), kinds[dtype], stretch,
-                                         work.data_ptr(), stretches, total_ptr, norms_ptr, coef_ptr, scale, limit,
-                                         device, hip._stream(first)), "netop_grad_norm")
+    table = array("Q", ptrs + ns)
+    at = table.buffer_info()[0]
+    hip._check((hip._lib or hip.lib()).netop_grad_norm(at, at + 8 * len(ns), len(ns), kinds[dtype], stretch,
+                                                       work.data_ptr(), stretches, total_ptr, norms_ptr, coef_ptr,
+                                                       scale, limit, device, hip._raw_stream(device)), "netop_grad_norm")
 
 
 class AdamW:
@@ -133,7 +141,7 @@ class AdamW:
     def __init__(self, params, *, lr, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.01, state_bits=32, seed=0):
         import torch
 
-        kinds = _dtypes()
+        kinds = _KINDS or _kinds()
         self.params = list(params)
         if not self.params:
             raise ValueError("no parameters")
@@ -241,14 +249,14 @@ class AdamW:
             raise ValueError(f"{len(self.params)} gradients expected, got {len(grads)}")
         if [p.data_ptr() for p in self.params] != self._ptrs:
             raise ValueError("a parameter has moved since the optimizer was made")
-        device, gtype, ptrs = self._index, None, array("Q")
+        device, gtype, ptrs = self._index, None, []
         for g, shape in zip(grads, self._shapes):
             if g is None:
                 ptrs.append(0)
                 continue
             if gtype is None:
                 gtype = g.dtype
-            if g.dtype != gtype:
+            if g.dtype is not gtype:
                 raise ValueError(f"gradients must have one type: {gtype} and {g.dtype}")
             if g.shape != shape:
                 raise ValueError(f"a gradient of shape {tuple(g.shape)} for a parameter of shape {tuple(shape)}")
@@ -259,13 +267,13 @@ class AdamW:
             ptrs.append(g.data_ptr())
         if gtype is None:
             return
-        kinds = _dtypes()
+        kinds = _KINDS or _kinds()
         if gtype not in kinds:
             raise ValueError(f"gradients: expected fp32, bf16 or fp16, got {gtype}")
         if not math.isfinite(scale):
             raise ValueError("scale must be finite")
         coef_ptr = 0 if coef is None else _one(coef, torch.float32, device, "coef")
-        (b1, b2), L, stream = self.betas, hip.lib(), hip._stream(self._table)
+        (b1, b2), L, stream = self.betas, hip._lib or hip.lib(), hip._raw_stream(device)
         step_ptr = _one(step, torch.int64, device, "step") if isinstance(step, torch.Tensor) else 0
         lr_ptr = _one(lr, torch.float32, device, "lr") if isinstance(lr, torch.Tensor) else 0
         t = 1 if step_ptr else int(step)
@@ -284,7 +292,8 @@ class AdamW:
             hip._check(L.netop_adamw_hyper(on_device, _HYPER.pack(*hyper), b1, b2, rate, self.weight_decay, self.seed,
                                            lr_ptr, step_ptr, t, device, stream), "netop_adamw_hyper")
         eight = self.state_bits == 8
-        at = ptrs.buffer_info()[0]
+        table = array("Q", ptrs)
+        at = table.buffer_info()[0]
         for a, b, chunks, n in self._launches:
             if n == 0:
                 continue  # nothing but empty tensors

@@ -31,35 +31,40 @@ _OVERLAP = -1
 _NO_INPUTS = [0] * (MAX_SRCS + 1)
 
 
-def _dtypes():
+def _kinds():
+    """Type codes and e4m3, once torch is there (the package is imported without it too)."""
+    global _KINDS
     import torch
 
-    return {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+    _KINDS = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}, torch.float32, torch.float8_e4m3fn
+    return _KINDS
+
+
+_KINDS = None
 
 
 def _pitch(t, shape, dtype, what, written=False):
     """The row stride of ``t`` in elements, after its checks."""
-    if t.dtype != dtype:
+    if t.dtype is not dtype:
         raise ValueError(f"{what}: expected {dtype}, got {t.dtype}")
     if t.shape != shape:
         raise ValueError(f"{what}: expected shape {tuple(shape)}, got {tuple(t.shape)}")
     cols = shape[-1]
-    if len(shape) == 2:
-        pitch, inner = t.stride()
-        if inner != 1 and cols > 1:
-            raise ValueError(f"{what}: the last dimension must be contiguous")
-        if written and pitch < cols and shape[0] > 1:
-            raise ValueError(f"{what}: its rows overlap")
-    else:
+    if len(shape) != 2:
         if not t.is_contiguous():
             raise ValueError(f"{what}: only 2-D tensors may have strides")
-        pitch = cols
+        return cols
+    pitch, inner = t.stride()
+    if inner != 1 and cols > 1:
+        raise ValueError(f"{what}: the last dimension must be contiguous")
+    if written and pitch < cols and shape[0] > 1:
+        raise ValueError(f"{what}: its rows overlap")
     return pitch
 
 
-def _flat(t, shape, dtypes, what):
-    if t.dtype not in dtypes:
-        raise ValueError(f"{what}: expected {' or '.join(str(d) for d in dtypes)}, got {t.dtype}")
+def _flat(t, shape, dtype, other, what):
+    if t.dtype is not dtype and t.dtype is not other:
+        raise ValueError(f"{what}: expected {dtype}{'' if other is dtype else f' or {other}'}, got {t.dtype}")
     if t.shape != shape:
         raise ValueError(f"{what}: expected shape {tuple(shape)}, got {tuple(t.shape)}")
     if not t.is_contiguous():
@@ -67,11 +72,12 @@ def _flat(t, shape, dtypes, what):
 
 
 def _on_one_device(device, tensors):
-    if device < 0 or any(t is not None and t.get_device() != device for t in tensors):
-        raise ValueError("every tensor must be on one CUDA device")
+    for t in tensors:
+        if t.get_device() != device or device < 0:
+            raise ValueError("every tensor must be on one CUDA device")
 
 
-def _checked(rc, what):
+def _failed(rc, what):
     if rc == _OVERLAP:
         raise ValueError("an output overlaps another tensor of the call (an output may replace an input of its type "
                          "element on element, and nothing else)")
@@ -98,9 +104,7 @@ def add_rms_norm(srcs, weight, out, *, residual=None, residual_out=None, rstd=No
     Sums and statistics are fp32; ``out`` comes from the unrounded sum and is rounded once.  An
     infinity or NaN in a row makes that row (in 8 bits: its scale) NaN or infinite and no other.
     """
-    import torch
-
-    kinds = _dtypes()
+    kinds, f32, e4m3 = _KINDS or _kinds()
     if not 1 <= len(srcs) <= MAX_SRCS:
         raise ValueError(f"1..{MAX_SRCS} partial sums")
     dtype, shape, device = srcs[0].dtype, out.shape, out.get_device()
@@ -110,38 +114,51 @@ def add_rms_norm(srcs, weight, out, *, residual=None, residual_out=None, rstd=No
         raise ValueError(f"out: expected (..., cols) with 1..{MAX_COLS} columns, got shape {tuple(shape)}")
     if not eps >= 0:
         raise ValueError("eps must not be negative")
-    cols = shape[-1]
-    rows = out.numel() // cols
-    kind, groups = 0, shape[:-1]
-    if out.dtype == torch.float8_e4m3fn:
+    cols, leading = shape[-1], shape[:-1]
+    kind = scales_ptr = h_ptr = h_pitch = rstd_ptr = 0
+    if out.dtype is e4m3:
         if scales is None:
             raise ValueError("an e4m3 output needs scales")
-        kind = 1 if scales.dim() == len(groups) else 2
-        _flat(scales, groups if kind == 1 else groups + (-(-cols // GROUP),), (torch.float32,), "scales")
+        kind = 1 if scales.dim() == len(leading) else 2
+        _flat(scales, leading if kind == 1 else leading + (-(-cols // GROUP),), f32, f32, "scales")
+        scales_ptr = scales.data_ptr()
     elif scales is not None:
         raise ValueError("scales belong to an e4m3 output")
-    out_pitch = _pitch(out, shape, out.dtype if kind else dtype, "out", True)
-    ptrs, pitches = [], []
-    for t in srcs:
-        pitches.append(_pitch(t, shape, dtype, "partial sum"))
-        ptrs.append(t.data_ptr())
+    out_pitch = _pitch(out, shape, e4m3 if kind else dtype, "out", True)
+    tensors = [*srcs, weight]
+    pitches = [_pitch(t, shape, dtype, "partial sum") for t in srcs]
+    ptrs = [t.data_ptr() for t in srcs]
     if residual is not None:
         pitches.append(_pitch(residual, shape, dtype, "residual"))
         ptrs.append(residual.data_ptr())
-    h_pitch = 0 if residual_out is None else _pitch(residual_out, shape, dtype, "residual_out", True)
-    _flat(weight, (cols,), (dtype, torch.float32), "weight")
+        tensors.append(residual)
+    if residual_out is not None:
+        h_pitch, h_ptr = _pitch(residual_out, shape, dtype, "residual_out", True), residual_out.data_ptr()
+        tensors.append(residual_out)
+    _flat(weight, (cols,), dtype, f32, "weight")
     if rstd is not None:
-        _flat(rstd, groups, (torch.float32,), "rstd")
-    _on_one_device(device, (*srcs, weight, residual, residual_out, rstd, scales))
-    if rows == 0:
-        return
+        _flat(rstd, leading, f32, f32, "rstd")
+        rstd_ptr = rstd.data_ptr()
+        tensors.append(rstd)
+    if scales_ptr:
+        tensors.append(scales)
+    _on_one_device(device, tensors)
+    rows = out.numel() // cols
+    if rows:
+        _launch(ptrs, pitches, weight.data_ptr(), out.data_ptr(), out_pitch, h_ptr, h_pitch, rstd_ptr, scales_ptr, rows,
+                cols, kinds[dtype], weight.dtype is f32, kind, device, eps)
+
+
+def _launch(ptrs, pitches, weight, out, out_pitch, h, h_pitch, rstd, scales, rows, cols, dtype, weight_f32, kind, device,
+            eps):
+    """The call into the library, on addresses (inputs may be a peer's memory)."""
     n = len(ptrs)
     pad = _NO_INPUTS[n:]
-    block = _FORWARD.pack(*ptrs, *pad, *pitches, *pad, weight.data_ptr(), out.data_ptr(), out_pitch,
-                          0 if residual_out is None else residual_out.data_ptr(), h_pitch,
-                          0 if rstd is None else rstd.data_ptr(), 0 if scales is None else scales.data_ptr(), rows,
-                          cols, n, kinds[dtype], weight.dtype == torch.float32, kind, device, eps, 0)
-    _checked(hip.lib().netop_add_rms_norm(block, hip._stream(out)), "netop_add_rms_norm")
+    block = _FORWARD.pack(*ptrs, *pad, *pitches, *pad, weight, out, out_pitch, h, h_pitch, rstd, scales, rows, cols, n,
+                          dtype, weight_f32, kind, device, eps, 0)
+    rc = (hip._lib or hip.lib()).netop_add_rms_norm(block, hip._raw_stream(device))
+    if rc:
+        _failed(rc, "netop_add_rms_norm")
 
 
 def add_rms_norm_backward(dy, h, weight, rstd, dh, dweight, *, dresidual=None) -> None:
@@ -156,7 +173,7 @@ def add_rms_norm_backward(dy, h, weight, rstd, dh, dweight, *, dresidual=None) -
     """
     import torch
 
-    kinds = _dtypes()
+    kinds, f32, _ = _KINDS or _kinds()
     dtype, shape, device = dy.dtype, dy.shape, dy.get_device()
     if dtype not in kinds:
         raise ValueError(f"dy: expected fp32, bf16 or fp16, got {dtype}")
@@ -168,16 +185,20 @@ def add_rms_norm_backward(dy, h, weight, rstd, dh, dweight, *, dresidual=None) -
     h_pitch = _pitch(h, shape, dtype, "h")
     dh_pitch = _pitch(dh, shape, dtype, "dh", True)
     dres_pitch = 0 if dresidual is None else _pitch(dresidual, shape, dtype, "dresidual")
-    _flat(weight, (cols,), (dtype, torch.float32), "weight")
-    _flat(rstd, shape[:-1], (torch.float32,), "rstd")
-    _flat(dweight, (cols,), (weight.dtype, torch.float32), "dweight")
-    _on_one_device(device, (h, dresidual, weight, rstd, dh, dweight))
-    L = hip.lib()
+    _flat(weight, (cols,), dtype, f32, "weight")
+    _flat(rstd, shape[:-1], f32, f32, "rstd")
+    _flat(dweight, (cols,), weight.dtype, f32, "dweight")
+    tensors = [h, weight, rstd, dh, dweight]
+    if dresidual is not None:
+        tensors.append(dresidual)
+    _on_one_device(device, tensors)
+    L = hip._lib or hip.lib()
     parts = L.netop_norm_backward_parts(rows, cols)
-    partial = torch.empty(parts * cols, dtype=torch.float32, device=dy.device)
+    partial = torch.empty(parts * cols, dtype=f32, device=dy.device)
     block = _BACKWARD.pack(dy.data_ptr(), dy_pitch, h.data_ptr(), h_pitch,
                            0 if dresidual is None else dresidual.data_ptr(), dres_pitch, weight.data_ptr(),
                            rstd.data_ptr(), dh.data_ptr(), dh_pitch, dweight.data_ptr(), partial.data_ptr(), rows,
-                           cols, parts, kinds[dtype], weight.dtype == torch.float32, dweight.dtype == torch.float32,
-                           device)
-    _checked(L.netop_add_rms_norm_backward(block, hip._stream(dy)), "netop_add_rms_norm_backward")
+                           cols, parts, kinds[dtype], weight.dtype is f32, dweight.dtype is f32, device)
+    rc = L.netop_add_rms_norm_backward(block, hip._raw_stream(device))
+    if rc:
+        _failed(rc, "netop_add_rms_norm_backward")

@@ -62,35 +62,48 @@ struct NormBackwardParams {
 };
 static_assert(sizeof(NormParams) == 240 && sizeof(NormBackwardParams) == 128, "ops/norm.py packs these");
 
-// The sum of x over the TPR threads of a row, in every one of them.  `red`: the row's TPR / 64 floats, which
-// the workgroup has not read since its last barrier.
+// A row's threads: TPR of them, several rows a workgroup, or (TPR = 0) the whole workgroup, whose size
+// then follows from the width: no wavefront idles because a width is no power of two.
+template <int TPR>
+struct Threads {
+    static constexpr int kBlock = TPR ? 256 : 1024;  // at most
+    static constexpr int kRows = TPR ? 256 / TPR : 1;
+    static constexpr bool kAlone = TPR && TPR <= 64;  // a row lies within a wavefront: no barriers
+    static constexpr int kSlots = TPR ? 4 : 16;       // wavefronts of a workgroup
+    __device__ static __forceinline__ int per_row() { return TPR ? TPR : int(blockDim.x); }
+    __device__ static __forceinline__ int mine() { return TPR ? int(threadIdx.x) % TPR : int(threadIdx.x); }
+    __device__ static __forceinline__ int row() { return TPR ? int(threadIdx.x) / TPR : 0; }
+};
+
+// The sum (the maximum) of x over a row's threads, in every one of them.  `red`: a float for each
+// wavefront of the workgroup, which nobody has read since the last barrier.
 template <int TPR>
 __device__ __forceinline__ float row_sum(float x, float* red) {
-    x = lanes_sum<(TPR < 64 ? TPR : 64)>(x);
-    if constexpr (TPR > 64) {
-        if ((threadIdx.x & 63) == 0) red[threadIdx.x % TPR >> 6] = x;
+    using Th = Threads<TPR>;
+    x = lanes_sum<(Th::kAlone ? TPR : 64)>(x);
+    if constexpr (!Th::kAlone) {
+        if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = x;
         __syncthreads();
-        x = 0;
-#pragma unroll
-        for (int i = 0; i < TPR / 64; ++i) x += red[i];
+        const int waves = Th::per_row() / 64, first = Th::row() * waves, i = threadIdx.x & 15;
+        x = lanes_sum<16>(i < waves ? red[first + i] : 0.0f);
     }
     return x;
 }
 template <int TPR>
 __device__ __forceinline__ float row_max(float x, float* red) {
-    x = lanes_max<(TPR < 64 ? TPR : 64), true>(x);
-    if constexpr (TPR > 64) {
-        if ((threadIdx.x & 63) == 0) red[threadIdx.x % TPR >> 6] = x;
+    using Th = Threads<TPR>;
+    x = lanes_max<(Th::kAlone ? TPR : 64), true>(x);
+    if constexpr (!Th::kAlone) {
+        if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = x;
         __syncthreads();
-        x = red[0];
-#pragma unroll
-        for (int i = 1; i < TPR / 64; ++i) x = x > red[i] || x != x ? x : red[i];
+        const int waves = Th::per_row() / 64, first = Th::row() * waves, i = threadIdx.x & 15;
+        x = lanes_max<16, true>(i < waves ? red[first + i] : 0.0f);
     }
     return x;
 }
 
-// Vectors of a row.  TPR threads hold it, VPT vectors of 8 columns each: vector k of thread t is columns
-// 8 (k TPR + t) and on.  One that would end behind the row is the row's last eight columns instead: every
+// Vectors of a row.  Its n threads hold VPT vectors of 8 columns each: vector k of thread t is columns
+// 8 (k n + t) and on.  One that would end behind the row is the row's last eight columns instead: every
 // load and store stays one instruction without a branch, columns that two threads hold come out the same
 // in both, and sums count them once (`twice` columns are left out).  Taking such a vector element by
 // element made a row of 5004 columns a third slower than one of 5008.  Rows have 8 columns at least.
@@ -105,13 +118,13 @@ struct At {
     }
 };
 
-template <class T, int TPR, int VPT, bool WHOLE, bool STREAM>
+template <class T, int VPT, bool WHOLE, bool STREAM>
 struct Row {
     Vec<T, 8> v[VPT];
-    __device__ __forceinline__ void load(const T* p, int t, int cols) {
+    __device__ __forceinline__ void load(const T* p, int t, int n, int cols) {
 #pragma unroll
         for (int k = 0; k < VPT; ++k) {
-            const At<WHOLE> at(k * TPR + t, cols);
+            const At<WHOLE> at(k * n + t, cols);
             if (at.in) v[k] = STREAM ? Wide<T, 8>::stream(p + at.c) : Wide<T, 8>::load(p + at.c);
         }
     }
@@ -139,52 +152,51 @@ __device__ __forceinline__ float larger(float x, float y) { return x > y || x !=
 
 // AHEAD inputs are on their way together: with peer pointers each is an xGMI round trip.
 template <class T, int TPR, int VPT, int AHEAD, bool E4M3, bool WHOLE, bool STREAM>
-__global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void norm_kernel(NormParams a) {
-    constexpr int kRows = TPR < 256 ? 256 / TPR : 1;
-    __shared__ float red[2][TPR < 64 ? 1 : TPR / 64 * kRows];
-    const uint64_t row = uint64_t(blockIdx.x) * kRows + threadIdx.x / TPR;
+__global__ __launch_bounds__(Threads<TPR>::kBlock) void norm_kernel(NormParams a) {
+    using Th = Threads<TPR>;
+    __shared__ float red[2][Th::kSlots];
+    const uint64_t row = uint64_t(blockIdx.x) * Th::kRows + Th::row();
     const bool here = row < a.rows;
-    if (TPR <= 64 && !here) return;  // all threads of a row, and rows of a wavefront or less meet no barrier
-    const int t = threadIdx.x % TPR;
+    if (Th::kAlone && !here) return;  // all threads of the row
+    const int t = Th::mine(), n = Th::per_row();
     const int cols = here ? a.cols : 0;
     Vec<float, 8> h[VPT];
 #pragma unroll
     for (int k = 0; k < VPT; ++k) h[k] = 0.0f;
     for (int s0 = 0; s0 < a.n_in; s0 += AHEAD) {
-        Row<T, TPR, VPT, WHOLE, STREAM> in[AHEAD];
+        Row<T, VPT, WHOLE, STREAM> in[AHEAD];
 #pragma unroll
         for (int s = 0; s < AHEAD; ++s)
-            if (s0 + s < a.n_in) in[s].load(static_cast<const T*>(a.in[s0 + s]) + int64_t(row) * a.in_stride[s0 + s], t, cols);
+            if (s0 + s < a.n_in) in[s].load(static_cast<const T*>(a.in[s0 + s]) + int64_t(row) * a.in_stride[s0 + s], t, n, cols);
 #pragma unroll
         for (int s = 0; s < AHEAD; ++s)
             if (s0 + s < a.n_in) {
 #pragma unroll
                 for (int k = 0; k < VPT; ++k)
-                    if (At<WHOLE>(k * TPR + t, cols).in) h[k] += widen<T, 8>(in[s].v[k]);
+                    if (At<WHOLE>(k * n + t, cols).in) h[k] += widen<T, 8>(in[s].v[k]);
             }
     }
     float ss = 0;
 #pragma unroll
     for (int k = 0; k < VPT; ++k) {
-        const At<WHOLE> at(k * TPR + t, cols);
+        const At<WHOLE> at(k * n + t, cols);
         if (at.in) ss = dot8(h[k], h[k], at.twice, ss);
     }
-    const int slot = TPR < 64 ? 0 : int(threadIdx.x) / TPR * (TPR / 64);
-    ss = row_sum<TPR>(ss, red[0] + slot);
+    ss = row_sum<TPR>(ss, red[0]);
     const float rstd = 1.0f / sqrtf(ss / float(a.cols) + a.eps);
     if (a.rstd && t == 0 && here) a.rstd[row] = rstd;
     if (a.h) {  // after the reduction: every thread of the row has read its inputs, which h may replace
         T* p = static_cast<T*>(a.h) + int64_t(row) * a.h_stride;
 #pragma unroll
         for (int k = 0; k < VPT; ++k) {
-            const At<WHOLE> at(k * TPR + t, cols);
+            const At<WHOLE> at(k * n + t, cols);
             if (at.in) Wide<T, 8>::store(p + at.c, narrow<T, 8>(h[k]));
         }
     }
     float amax = 0;
 #pragma unroll
     for (int k = 0; k < VPT; ++k) {
-        const At<WHOLE> at(k * TPR + t, cols);
+        const At<WHOLE> at(k * n + t, cols);
         if (at.in) h[k] = h[k] * rstd * weights8<T>(a.weight, a.weight_f32, at.c);
         if constexpr (E4M3) {
 #pragma unroll
@@ -195,7 +207,7 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void norm_kernel(NormParams 
         T* p = static_cast<T*>(a.out) + int64_t(row) * a.out_stride;
 #pragma unroll
         for (int k = 0; k < VPT; ++k) {
-            const At<WHOLE> at(k * TPR + t, cols);
+            const At<WHOLE> at(k * n + t, cols);
             if (at.in) Wide<T, 8>::store(p + at.c, narrow<T, 8>(h[k]));
         }
     } else {
@@ -203,18 +215,18 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void norm_kernel(NormParams 
         const bool by_group = a.out_kind == kGroupScale;
         const int groups = (cols + kGroup - 1) / kGroup;
         if (!by_group) {
-            amax = row_max<TPR>(amax, red[1] + slot);
+            amax = row_max<TPR>(amax, red[1]);
             if (t == 0 && here) a.scales[row] = amax < kTiny ? 0.0f : amax / kE4m3Max;
         }
 #pragma unroll
         for (int k = 0; k < VPT; ++k) {
-            const At<WHOLE> at(k * TPR + t, cols);
+            const At<WHOLE> at(k * n + t, cols);
             if (by_group) {  // 16 neighbouring threads hold a group
                 amax = 0;
 #pragma unroll
                 for (int j = 0; j < 8; ++j) amax = j >= at.twice ? larger(amax, fabsf(h[k][j])) : amax;
-                amax = lanes_max<(TPR < 16 ? TPR : 16), true>(amax);
-                if ((t & 15) == 0 && at.in) a.scales[row * groups + (k * TPR + t) / 16] = amax < kTiny ? 0.0f : amax / kE4m3Max;
+                amax = lanes_max<(TPR == 8 ? 8 : 16), true>(amax);
+                if ((t & 15) == 0 && at.in) a.scales[row * groups + (k * n + t) / 16] = amax < kTiny ? 0.0f : amax / kE4m3Max;
             }
             const float inv = amax < kTiny ? 0.0f : kE4m3Max / amax;
             if (!at.in) continue;
@@ -277,79 +289,82 @@ __global__ __launch_bounds__(256) void narrow_norm_kernel(NormParams a) {
 // Each row's share of dweight stays in the registers of the thread that holds those columns; a
 // workgroup walks rows in steps of the grid, adds up its rows' shares and writes one partial row,
 // and dweight_kernel adds those up: a fixed order, no atomics, the same bits every time.  With four
-// vectors a thread 128 registers do not hold a row beside dweight, and it is read a second time, out of
-// the caches.  (Fetching the next row ahead costs as many registers and gained nothing: 53 against 51 us
+// vectors of fp32 a thread 128 registers do not hold a row beside dweight, and it is read a second time, out
+// of the caches.  (Fetching the next row ahead costs as many registers and gained nothing: 53 against 51 us
 // at 8192 x 4096.)
 template <class T, int TPR, int VPT, bool WHOLE, bool STREAM>
-__global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void norm_backward_kernel(NormBackwardParams a) {
-    constexpr int kRows = TPR < 256 ? 256 / TPR : 1;
-    constexpr bool kTwice = VPT == 4;
-    __shared__ float red[2][TPR < 64 ? 1 : TPR / 64 * kRows];
-    const int t = threadIdx.x % TPR, r = int(threadIdx.x) / TPR;
-    const int slot = TPR < 64 ? 0 : r * (TPR / 64);
+__global__ __launch_bounds__(Threads<TPR>::kBlock) void norm_backward_kernel(NormBackwardParams a) {
+    using Th = Threads<TPR>;
+    constexpr int kRows = Th::kRows;
+    constexpr bool kTwice = VPT == 4 && sizeof(T) == 4, kWeights = VPT <= 2;
+    __shared__ float red[2][Th::kSlots];
+    const int t = Th::mine(), n = Th::per_row(), r = Th::row();
     const uint64_t first = uint64_t(blockIdx.x) * kRows, walk = uint64_t(gridDim.x) * kRows;
     Vec<float, 8> dw[VPT], weight[VPT];
 #pragma unroll
     for (int k = 0; k < VPT; ++k) {
         dw[k] = 0.0f;
-        const At<WHOLE> at(k * TPR + t, a.cols);
-        if (!kTwice && at.in) weight[k] = weights8<T>(a.weight, a.weight_f32, at.c);
+        const At<WHOLE> at(k * n + t, a.cols);
+        if (kWeights && at.in) weight[k] = weights8<T>(a.weight, a.weight_f32, at.c);
     }
     int turn = 0;
     // Rows that share barriers take as many turns as the workgroup's first.
-    for (uint64_t base = first, row = first + r; (TPR <= 64 ? row : base) < a.rows; base += walk, row += walk, turn ^= 1) {
+    for (uint64_t base = first, row = first + r; (Th::kAlone ? row : base) < a.rows; base += walk, row += walk, turn ^= 1) {
         const int cols = row < a.rows ? a.cols : 0;
         const float rstd = cols ? a.rstd[row] : 0.0f;
         const T* dy = static_cast<const T*>(a.dy) + int64_t(row) * a.dy_stride;
         const T* hp = static_cast<const T*>(a.h) + int64_t(row) * a.h_stride;
         const T* rp = a.dres ? static_cast<const T*>(a.dres) + int64_t(row) * a.dres_stride : nullptr;
         T* dh = static_cast<T*>(a.dh) + int64_t(row) * a.dh_stride;
-        Row<T, TPR, VPT, WHOLE, STREAM> raw_g, raw_h, raw_r;
+        Row<T, VPT, WHOLE, STREAM> raw_g, raw_h, raw_r;
         if constexpr (!kTwice) {
-            raw_g.load(dy, t, cols);
-            raw_h.load(hp, t, cols);
-            if (rp) raw_r.load(rp, t, cols);
+            raw_g.load(dy, t, n, cols);
+            raw_h.load(hp, t, n, cols);
+            if (rp) raw_r.load(rp, t, n, cols);
         }
-        Vec<float, 8> g[VPT];
         float dot = 0;
 #pragma unroll
         for (int k = 0; k < VPT; ++k) {
-            const At<WHOLE> at(k * TPR + t, cols);
+            const At<WHOLE> at(k * n + t, cols);
             if (at.in) {
                 if constexpr (kTwice) {
                     raw_g.v[k] = Wide<T, 8>::load(dy + at.c);
                     raw_h.v[k] = Wide<T, 8>::load(hp + at.c);
                 }
-                g[k] = widen<T, 8>(raw_g.v[k]);
-                const Vec<float, 8> h = widen<T, 8>(raw_h.v[k]);
-                dw[k] += g[k] * h * rstd;
-                if constexpr (kTwice) weight[k] = weights8<T>(a.weight, a.weight_f32, at.c);
-                g[k] *= weight[k];
-                dot = dot8(g[k], h, at.twice, dot);
+                if constexpr (!kWeights) weight[k] = weights8<T>(a.weight, a.weight_f32, at.c);
+                const Vec<float, 8> g = widen<T, 8>(raw_g.v[k]), h = widen<T, 8>(raw_h.v[k]);
+                dw[k] += g * h * rstd;
+                dot = dot8(g * weight[k], h, at.twice, dot);
             }
-            if constexpr (kTwice) asm volatile("" ::: "memory");  // holds back the next vector's loads
+            if constexpr (!kWeights) asm volatile("" ::: "memory");  // holds back the next vector's loads
         }
-        dot = row_sum<TPR>(dot, red[turn] + slot);
+        dot = row_sum<TPR>(dot, red[turn]);
         const float back = rstd * rstd * rstd * (dot / float(a.cols));
+        Vec<T, 8> d[VPT];
 #pragma unroll
         for (int k = 0; k < VPT; ++k) {
-            const At<WHOLE> at(k * TPR + t, cols);
+            const At<WHOLE> at(k * n + t, cols);
             if (at.in) {
                 if constexpr (kTwice) {
-                    g[k] = widen<T, 8>(Wide<T, 8>::load(dy + at.c)) * weights8<T>(a.weight, a.weight_f32, at.c);
+                    raw_g.v[k] = Wide<T, 8>::load(dy + at.c);
                     raw_h.v[k] = Wide<T, 8>::load(hp + at.c);
                     if (rp) raw_r.v[k] = Wide<T, 8>::load(rp + at.c);
                 }
-                g[k] = rstd * g[k] - widen<T, 8>(raw_h.v[k]) * back;
-                if (rp) g[k] += widen<T, 8>(raw_r.v[k]);
+                if constexpr (!kWeights) weight[k] = weights8<T>(a.weight, a.weight_f32, at.c);
+                Vec<float, 8> x = rstd * (widen<T, 8>(raw_g.v[k]) * weight[k]) - widen<T, 8>(raw_h.v[k]) * back;
+                if (rp) x += widen<T, 8>(raw_r.v[k]);
+                d[k] = narrow<T, 8>(x);
+                if constexpr (!kTwice) Wide<T, 8>::store(dh + at.c, d[k]);
             }
-            if constexpr (kTwice) asm volatile("" ::: "memory");
+            if constexpr (!kWeights) asm volatile("" ::: "memory");
         }
-        if constexpr (kTwice) __syncthreads();  // dh may be where two threads have just read the same columns
+        if constexpr (kTwice) {
+            __syncthreads();  // dh may be where two threads have just read the same columns
 #pragma unroll
-        for (int k = 0; k < VPT; ++k) {
-            const At<WHOLE> at(k * TPR + t, cols);
-            if (at.in) Wide<T, 8>::store(dh + at.c, narrow<T, 8>(g[k]));
+            for (int k = 0; k < VPT; ++k) {
+                const At<WHOLE> at(k * n + t, cols);
+                if (at.in) Wide<T, 8>::store(dh + at.c, d[k]);
+            }
         }
     }
     if constexpr (kRows > 1) {
@@ -362,7 +377,7 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void norm_backward_kernel(No
     }
 #pragma unroll
     for (int k = 0; k < VPT; ++k) {
-        const At<WHOLE> at(k * TPR + t, a.cols);
+        const At<WHOLE> at(k * n + t, a.cols);
         if (at.in) Wide<float, 8>::store(a.partial + uint64_t(blockIdx.x) * a.cols + at.c, dw[k]);
     }
 }
@@ -456,27 +471,30 @@ __global__ __launch_bounds__(1024) void dweight_kernel(const float* __restrict__
 
 // ---- which threads hold a row -------------------------------------------------------------------
 struct Shape {
-    int tpr, vpt;
+    int tpr, vpt, block;
 };
 
-// One vector a thread up to 4096 columns: fewest registers, most rows in flight.  Beyond, a row of two
-// vectors a thread leaves each CU two workgroups (16384 x 8192 bf16 to e4m3: 176 us with 512 threads, 202 with
-// 1024), while few rows end sooner spread wider (64 x 8192, 8 partial sums: 5.3 us with 1024, 6.6 with 512).
+// One vector a thread up to 4096 columns: fewest registers, most rows in flight.  Beyond, rows of two
+// vectors a thread leave each CU more workgroups (16384 x 8192 bf16 to e4m3: 176 us with 512 threads, 202 with
+// 1024), while few rows end sooner spread wider (64 x 8192, 8 partial sums: 5.0 us with 1024, 6.4 with 512).
 Shape shape_for(int cols, uint64_t rows) {
     const int vecs = (cols + 7) / 8;
-    for (int tpr = 8; tpr <= 512; tpr *= 2)
-        if (vecs <= tpr) return {tpr, 1};
-    if (vecs <= 1024) return rows > 1024 ? Shape{512, 2} : Shape{1024, 1};
-    return vecs <= 2048 ? Shape{1024, 2} : Shape{1024, 4};
+    for (int tpr = 8; tpr <= 128; tpr *= 2)
+        if (vecs <= tpr) return {tpr, 1, 256};
+    const int vpt = vecs <= 512 || (vecs <= 1024 && rows <= 1024) ? 1 : vecs <= 2048 ? 2 : 4;
+    // Four vectors a thread need every wavefront there is room for (backward 3000 x 20000: 142 us, 198 with 640).
+    return {0, vpt, vpt == 4 ? 1024 : ((vecs + vpt - 1) / vpt + 63) / 64 * 64};
 }
 
-// Workgroups of the backward pass, each with a partial row of dweight: enough to fill the chip, few enough
-// that their rows cost little next to the data.
+// Workgroups of the backward pass, each with a partial row of dweight: as many as are at work together, and
+// few where rows are few, since a partial row costs two rows of fp32.  8192 x 4096 bf16: 512 50 us, 256 66,
+// 1024 57; 8192 x 7168 fp32: 256 172 us, 512 182; 1000 x 5003 bf16: 256 17.4 us, 512 21.7.
 int parts_for(int cols, uint64_t rows) {
-    const int tpr = cols < 8 ? 1 : shape_for(cols, rows).tpr;
-    const uint64_t at_once = tpr < 256 ? 256 / tpr : 1;
-    const uint64_t most = tpr < 256 ? 1024 : rows >= 2048 ? 512 : 256, need = (rows + at_once - 1) / at_once;
-    return int(need < most ? need : most);
+    const Shape s = shape_for(cols, rows);
+    const uint64_t at_once = cols < 8 ? 256 : s.tpr ? 256 / s.tpr : 1;
+    const uint64_t most = cols < 8 || s.tpr ? 1024 : rows >= 2048 && s.vpt == 1 && s.block <= 640 ? 512 : 256;
+    const uint64_t need = (rows + at_once - 1) / at_once, turns = (need + most - 1) / most;
+    return turns ? int((need + turns - 1) / turns) : 0;  // all of them as many turns: 333 rows are 167 times two
 }
 
 // Inputs of 64 MiB and more are read past the caches: they hardly lie there (256 MB) and will not be read
@@ -487,9 +505,9 @@ bool past_caches(uint64_t rows, int cols, int inputs) {
 }
 
 template <class T, int TPR, int VPT>
-void launch_norm(const NormParams& a, hipStream_t stream) {
-    constexpr int kRows = TPR < 256 ? 256 / TPR : 1, kMany = 8 / VPT > 2 ? 8 / VPT : 2;
-    const dim3 grid(unsigned((a.rows + kRows - 1) / kRows)), block(TPR < 256 ? 256 : TPR);
+void launch_norm(const NormParams& a, int block, hipStream_t stream) {
+    constexpr int kRows = Threads<TPR>::kRows, kMany = 8 / VPT > 2 ? 8 / VPT : 2;
+    const dim3 grid(unsigned((a.rows + kRows - 1) / kRows));
     const bool few = a.n_in <= 2, whole = a.cols % 8 == 0, eight = a.out_kind != kSame;
     constexpr bool kStreams = sizeof(T) == 2;
     const bool streams = kStreams && past_caches(a.rows, a.cols, a.n_in);
@@ -498,36 +516,31 @@ void launch_norm(const NormParams& a, hipStream_t stream) {
                    : streams ? eight ? norm_kernel<T, TPR, VPT, 2, true, true, kStreams> : norm_kernel<T, TPR, VPT, 2, false, true, kStreams>
                    : eight   ? norm_kernel<T, TPR, VPT, 2, true, true, false>
                              : norm_kernel<T, TPR, VPT, 2, false, true, false>;
-    hipLaunchKernelGGL(k, grid, block, 0, stream, a);
+    hipLaunchKernelGGL(k, grid, dim3(unsigned(block)), 0, stream, a);
 }
 
 template <class T, int TPR, int VPT>
-void launch_backward(const NormBackwardParams& a, hipStream_t stream) {
+void launch_backward(const NormBackwardParams& a, int block, hipStream_t stream) {
     constexpr bool kStreams = sizeof(T) == 2;
     const auto k = a.cols % 8 ? norm_backward_kernel<T, TPR, VPT, false, false>
                    : kStreams && past_caches(a.rows, a.cols, a.dres ? 3 : 2) ? norm_backward_kernel<T, TPR, VPT, true, kStreams>
                                                                             : norm_backward_kernel<T, TPR, VPT, true, false>;
-    hipLaunchKernelGGL(k, dim3(unsigned(a.parts)), dim3(TPR < 256 ? 256 : TPR), 0, stream, a);
+    hipLaunchKernelGGL(k, dim3(unsigned(a.parts)), dim3(unsigned(block)), 0, stream, a);
 }
 
-#define NETOP_FOR_SHAPE(s, CALL)                    \
-    do {                                            \
-        switch (s.tpr) {                            \
-            case 8: CALL(8, 1); break;              \
-            case 16: CALL(16, 1); break;            \
-            case 32: CALL(32, 1); break;            \
-            case 64: CALL(64, 1); break;            \
-            case 128: CALL(128, 1); break;          \
-            case 256: CALL(256, 1); break;          \
-            case 512:                               \
-                if (s.vpt == 1) CALL(512, 1);       \
-                else CALL(512, 2);                  \
-                break;                              \
-            default:                                \
-                if (s.vpt == 1) CALL(1024, 1);      \
-                else if (s.vpt == 2) CALL(1024, 2); \
-                else CALL(1024, 4);                 \
-        }                                           \
+#define NETOP_FOR_SHAPE(s, CALL)              \
+    do {                                      \
+        switch (s.tpr) {                      \
+            case 8: CALL(8, 1); break;        \
+            case 16: CALL(16, 1); break;      \
+            case 32: CALL(32, 1); break;      \
+            case 64: CALL(64, 1); break;      \
+            case 128: CALL(128, 1); break;    \
+            default:                          \
+                if (s.vpt == 1) CALL(0, 1);   \
+                else if (s.vpt == 2) CALL(0, 2); \
+                else CALL(0, 4);              \
+        }                                     \
     } while (0)
 
 template <class T>
@@ -537,7 +550,7 @@ void norm_of(const NormParams& a, hipStream_t stream) {
         return;
     }
     const Shape s = shape_for(a.cols, a.rows);
-#define CALL(TPR, VPT) launch_norm<T, TPR, VPT>(a, stream)
+#define CALL(TPR, VPT) launch_norm<T, TPR, VPT>(a, s.block, stream)
     NETOP_FOR_SHAPE(s, CALL);
 #undef CALL
 }
@@ -548,7 +561,7 @@ void backward_of(const NormBackwardParams& a, hipStream_t stream) {
         return;
     }
     const Shape s = shape_for(a.cols, a.rows);
-#define CALL(TPR, VPT) launch_backward<T, TPR, VPT>(a, stream)
+#define CALL(TPR, VPT) launch_backward<T, TPR, VPT>(a, s.block, stream)
     NETOP_FOR_SHAPE(s, CALL);
 #undef CALL
 }

@@ -25,7 +25,7 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kBlock = 256;          // elements that share a scale: 64 lanes x 4
-constexpr int kUnroll = 4;           // blocks a wavefront works on together
+constexpr int kUnroll = 2;           // blocks a wavefront works on together: 4 leave uneven ends (784 us for 755)
 constexpr int kChunk = kThreads / 64 * kUnroll * kBlock;  // elements of one workgroup
 constexpr int kMaxGrads = 440;       // gradient addresses that fit a launch's arguments (4 KiB)
 
@@ -64,13 +64,21 @@ struct Grads {
 static_assert(sizeof(StepParams) == 128 && sizeof(Hyper) == 40 && sizeof(Chunk) == 32, "ops/adamw.py packs these");
 static_assert(sizeof(StepParams) + sizeof(Grads) <= 4096, "kernel arguments");
 
-__device__ __forceinline__ uint32_t random32(uint64_t position, uint32_t key) {
-    uint32_t x = uint32_t(position) * 0x9E3779B1u ^ uint32_t(position >> 32) * 0x85EBCA77u ^ key;
-    x ^= x >> 15;
-    x *= 0x2C1B3C6Du;
-    x ^= x >> 12;
-    x *= 0x297A2D39u;
-    return x ^ (x >> 15);
+// Four random numbers, for the positions from a multiple of four on: one product reaches all of them.
+__device__ __forceinline__ Vec<uint32_t, 4> random4(uint64_t position, uint32_t key) {
+    constexpr uint32_t kLow = 0x9E3779B1u;
+    const uint32_t low = uint32_t(position) * kLow, high = uint32_t(position >> 32) * 0x85EBCA77u ^ key;
+    Vec<uint32_t, 4> r;
+#pragma unroll
+    for (uint32_t j = 0; j < 4; ++j) {
+        uint32_t x = (low + j * kLow) ^ high;
+        x ^= x >> 15;
+        x *= 0x2C1B3C6Du;
+        x ^= x >> 12;
+        x *= 0x297A2D39u;
+        r[j] = x ^ (x >> 15);
+    }
+    return r;
 }
 
 __host__ __device__ __forceinline__ uint32_t key_of(uint32_t seed, uint64_t step) {
@@ -87,18 +95,19 @@ __device__ __forceinline__ uint32_t stochastic_e4m3(float u, uint32_t rnd) {
     return u < 0x1p-6f ? small : normal;
 }
 
-template <class T>
-__device__ __forceinline__ Vec<float, 4> load4(const T* p, int n) {  // n elements, zeros behind
-    if (n >= 4) return widen<T, 4>(Wide<T, 4>::stream(p));
+// n of four elements, zeros behind; all of them where the chunk is whole.
+template <bool WHOLE, class T>
+__device__ __forceinline__ Vec<float, 4> load4(const T* p, int n) {
+    if (WHOLE || n >= 4) return widen<T, 4>(Wide<T, 4>::stream(p));
     Vec<float, 4> v = 0.0f;
 #pragma unroll
     for (int j = 0; j < 3; ++j)
         if (j < n) v[j] = float(p[j]);
     return v;
 }
-template <class T>
+template <bool WHOLE, class T>
 __device__ __forceinline__ void store4(T* p, const Vec<float, 4>& v, int n) {
-    if (n >= 4) {
+    if (WHOLE || n >= 4) {
         Wide<T, 4>::put(p, narrow<T, 4>(v));
         return;
     }
@@ -108,21 +117,12 @@ __device__ __forceinline__ void store4(T* p, const Vec<float, 4>& v, int n) {
 }
 
 // Products and sums are rounded one by one, not contracted: which way a state rounds hangs on the last
-// bit, and is to follow from the formulas alone, whatever compiled them.
-template <class P, class G, int BITS>
-__global__ __launch_bounds__(kThreads) void adamw_kernel(StepParams a, Grads grads) {
+// bit, and is to follow from the formulas alone, whatever compiled them.  The quotient in p's step decides
+// nothing and takes the hardware's reciprocal (1 ulp).
+template <class P, class G, int BITS, bool WHOLE>
+__device__ __forceinline__ void chunk_step(const StepParams& a, const Chunk& ch, const G* gp, const Hyper& hy, float coef) {
 #pragma clang fp contract(off)
     constexpr bool kMaster = sizeof(P) == 2;
-    const Chunk ch = a.chunks[blockIdx.x];
-    const G* gp = static_cast<const G*>(grads.at[ch.tensor]);
-    if (!gp) return;  // no gradient: the tensor keeps its value and states
-    const Hyper hy = a.on_device ? *a.on_device : a.hyper;
-    float coef = hy.scale;
-    if (a.coef) {
-        coef *= *a.coef;
-        if (!(fabsf(coef) < __builtin_inff())) return;  // the gradients overflowed: the step is left out
-    }
-    gp += ch.start;
     P* pp = reinterpret_cast<P*>(ch.p);
     const int lane = threadIdx.x & 63;
     const int base = (threadIdx.x >> 6) * (kUnroll * kBlock) + lane * 4;
@@ -132,10 +132,10 @@ __global__ __launch_bounds__(kThreads) void adamw_kernel(StepParams a, Grads gra
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u) {
         const int i = base + u * kBlock, n = ch.n - i;
-        if (i - lane * 4 >= ch.n) break;  // the whole block lies behind the tensor's end
+        if (!WHOLE && i - lane * 4 >= ch.n) break;  // the whole block lies behind the tensor's end
         const uint64_t at = ch.offset + i;
-        g[u] = load4(gp + i, n);
-        w[u] = kMaster ? load4(a.master + at, n) : load4(reinterpret_cast<const float*>(pp) + i, n);
+        g[u] = load4<WHOLE>(gp + i, n);
+        w[u] = kMaster ? load4<WHOLE>(a.master + at, n) : load4<WHOLE>(reinterpret_cast<const float*>(pp) + i, n);
         if constexpr (BITS == 32) {  // states are padded to whole blocks
             m[u] = Wide<float, 4>::stream(static_cast<const float*>(a.m) + at);
             v[u] = Wide<float, 4>::stream(static_cast<const float*>(a.v) + at);
@@ -149,7 +149,7 @@ __global__ __launch_bounds__(kThreads) void adamw_kernel(StepParams a, Grads gra
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u) {
         const int i = base + u * kBlock, n = ch.n - i;
-        if (i - lane * 4 >= ch.n) break;
+        if (!WHOLE && i - lane * 4 >= ch.n) break;
         const uint64_t at = ch.offset + i;
         if constexpr (BITS == 8) {
             m[u] = unpack_e4m3(mq[u]) * ms[u];
@@ -164,12 +164,12 @@ __global__ __launch_bounds__(kThreads) void adamw_kernel(StepParams a, Grads gra
             m[u][j] = hy.b1 * m[u][j] + hy.one_b1 * x;
             v[u][j] = hy.b2 * v[u][j] + hy.one_b2 * (x * x);
             root[j] = sqrtf(v[u][j]);
-            w[u][j] = w[u][j] * hy.decay - hy.alpha * m[u][j] / (root[j] * hy.rc2 + hy.eps);
+            w[u][j] = w[u][j] * hy.decay - hy.alpha * m[u][j] * __builtin_amdgcn_rcpf(root[j] * hy.rc2 + hy.eps);
             m_max = fmaxf(m_max, fabsf(m[u][j]));
             r_max = fmaxf(r_max, root[j]);
         }
-        if constexpr (kMaster) store4(a.master + at, w[u], n);
-        store4(pp + i, w[u], n);
+        if constexpr (kMaster) store4<WHOLE>(a.master + at, w[u], n);
+        store4<WHOLE>(pp + i, w[u], n);
         if constexpr (BITS == 32) {
             Wide<float, 4>::put(static_cast<float*>(a.m) + at, m[u]);
             Wide<float, 4>::put(static_cast<float*>(a.v) + at, v[u]);
@@ -180,13 +180,13 @@ __global__ __launch_bounds__(kThreads) void adamw_kernel(StepParams a, Grads gra
             const float r_scale = r_max < kTiny ? 0.0f : r_max * (1.0f / kE4m3Max);
             const float m_inv = m_max < kTiny ? 0.0f : 1.0f / m_scale;
             const float r_inv = r_max < kTiny ? 0.0f : 1.0f / r_scale;
+            const Vec<uint32_t, 4> rnd = random4(at, hy.key);
             uint32_t mw = 0, vw = 0;
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                const uint32_t rnd = random32(at + j, hy.key);
                 const float x = m[u][j], r = root[j];
-                uint32_t mc = stochastic_e4m3(fminf(fabsf(x) * m_inv, kE4m3Max), rnd & 0xffffu);
-                uint32_t vc = stochastic_e4m3(fminf(r * r_inv, kE4m3Max), rnd >> 16);
+                uint32_t mc = stochastic_e4m3(fminf(fabsf(x) * m_inv, kE4m3Max), rnd[j] & 0xffffu);
+                uint32_t vc = stochastic_e4m3(fminf(r * r_inv, kE4m3Max), rnd[j] >> 16);
                 if (vc == 0 && r * r_inv > 0) vc = 1;
                 mc = x != x ? 0x7fu : mc | (__float_as_uint(x) >> 24 & 0x80u);
                 vc = r != r ? 0x7fu : vc;
@@ -201,6 +201,23 @@ __global__ __launch_bounds__(kThreads) void adamw_kernel(StepParams a, Grads gra
             }
         }
     }
+}
+
+template <class P, class G, int BITS>
+__global__ __launch_bounds__(kThreads) void adamw_kernel(StepParams a, Grads grads) {
+    const Chunk ch = a.chunks[blockIdx.x];
+    const G* gp = static_cast<const G*>(grads.at[ch.tensor]);
+    if (!gp) return;  // no gradient: the tensor keeps its value and states
+    const Hyper hy = a.on_device ? *a.on_device : a.hyper;
+    float coef = hy.scale;
+    if (a.coef) {
+        coef *= *a.coef;
+        if (!(fabsf(coef) < __builtin_inff())) return;  // the gradients overflowed: the step is left out
+    }
+    if (ch.n == kChunk)
+        chunk_step<P, G, BITS, true>(a, ch, gp + ch.start, hy, coef);
+    else
+        chunk_step<P, G, BITS, false>(a, ch, gp + ch.start, hy, coef);
 }
 
 // The step's numbers where lr or step are on the device (a captured graph's are): 64 bits, since

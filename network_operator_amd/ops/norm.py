@@ -104,6 +104,13 @@ def add_rms_norm(srcs, weight, out, *, residual=None, residual_out=None, rstd=No
     Sums and statistics are fp32; ``out`` comes from the unrounded sum and is rounded once.  An
     infinity or NaN in a row makes that row (in 8 bits: its scale) NaN or infinite and no other.
     """
+    args = _arguments(srcs, weight, out, residual, residual_out, rstd, scales, eps)
+    if args:
+        _launch(*args)
+
+
+def _arguments(srcs, weight, out, residual, residual_out, rstd, scales, eps):
+    """:func:`_launch`'s arguments, after every check; ``None`` without rows."""
     kinds, f32, e4m3 = _KINDS or _kinds()
     if not 1 <= len(srcs) <= MAX_SRCS:
         raise ValueError(f"1..{MAX_SRCS} partial sums")
@@ -144,9 +151,10 @@ def add_rms_norm(srcs, weight, out, *, residual=None, residual_out=None, rstd=No
         tensors.append(scales)
     _on_one_device(device, tensors)
     rows = out.numel() // cols
-    if rows:
-        _launch(ptrs, pitches, weight.data_ptr(), out.data_ptr(), out_pitch, h_ptr, h_pitch, rstd_ptr, scales_ptr, rows,
-                cols, kinds[dtype], weight.dtype is f32, kind, device, eps)
+    if not rows:
+        return None
+    return (ptrs, pitches, weight.data_ptr(), out.data_ptr(), out_pitch, h_ptr, h_pitch, rstd_ptr, scales_ptr, rows, cols,
+            kinds[dtype], weight.dtype is f32, kind, device, eps)
 
 
 def _launch(ptrs, pitches, weight, out, out_pitch, h, h_pitch, rstd, scales, rows, cols, dtype, weight_f32, kind, device,

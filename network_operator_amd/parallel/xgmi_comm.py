@@ -12,6 +12,8 @@ construction (ring algorithms need many concurrent rings to do the same):
 chunk into every peer's output): xGMI read and write bandwidth differ, so both are measured.
 ``one_shot`` instead has every rank sum the whole message from all inputs (one phase, n-1 times
 the link traffic): the better choice for small messages, where phase overhead dominates.
+:meth:`XgmiAllReduce.all_reduce_norm` ends it with the residual's addition and the RMS norm of a
+tensor-parallel layer, in the kernel that reads the peers' partial sums.
 
 Each rank owns two *symmetric* buffers (input, output) allocated once, exported with HIP IPC
 and mapped by every peer (``native/hip/xgmi_comm.hip``).  Callers write the message into
@@ -44,7 +46,7 @@ import time
 import uuid
 from typing import List, Optional
 
-from ..ops import hip as H
+from ..ops import hip as H, norm as N
 
 ALGOS = ("two_shot", "two_shot_push", "one_shot")
 # Below this size one phase beats two: one_shot moves (n-1)x the bytes but pays one barrier
@@ -217,6 +219,39 @@ class XgmiAllReduce:
         H._check(L.netop_multi_copy(src, dst, len(peers), cb, self.wg_per_cu, s), "netop_multi_copy")
         self._sync_and_wait(stream)  # every chunk has arrived; nobody touches my buffers any more
         return self.output(numel)
+
+    def all_reduce_norm(self, weight, out, *, residual=None, residual_out=None, rstd=None, scales=None,
+                        eps: float = 1e-6, algo: str = "auto") -> None:
+        """:func:`~network_operator_amd.ops.norm.add_rms_norm` over every rank's partial sum: ``out``
+        (with ``residual_out``, ``rstd`` and ``scales``) is the normalised sum of all ranks'
+        ``input(out.numel())``, read as ``out``'s shape, and ``residual``, which every rank holds.
+        bf16; ``out`` bf16 or e4m3.  The same bits on every rank.
+
+        ``one_shot`` reads the peers' partial sums in the norm kernel, and the sum is never rounded
+        before it is normalised; it takes any number of elements.  The two-shot variants (see
+        :func:`choose_algo`) normalise :meth:`all_reduce`'s result, which is rounded to bf16 once."""
+        import torch
+
+        numel = out.numel()
+        if algo == "auto" and numel % 8:
+            algo = "one_shot"
+        if algo != "one_shot":
+            algo = choose_algo(numel, self.world, algo)
+        mine = self.input(numel).view(out.shape)
+        one_shot = algo == "one_shot" or self.world == 1
+        args = N._arguments([mine] * (self.world if one_shot else 1), weight, out, residual, residual_out, rstd, scales, eps)
+        if args is None:
+            return
+        if not one_shot:
+            reduced = self.all_reduce(numel, algo).view(out.shape)
+            N.add_rms_norm([reduced], weight, out, residual=residual, residual_out=residual_out, rstd=rstd,
+                           scales=scales, eps=eps)
+            return
+        args[0][:self.world] = self.peer_in  # in rank order, this rank's among them
+        stream = torch.cuda.current_stream(self.device)
+        self._sync_and_wait(stream)  # every partial sum is complete
+        N._launch(*args)
+        self._sync_and_wait(stream)  # nobody reads my partial sum any more
 
     def reduce_scatter(self, numel: int, offset: int = 0):
         """Rank d gets chunk d of the sum of every rank's ``input(offset + numel)[offset:]``

@@ -20,6 +20,7 @@ from __future__ import annotations
 import math
 import struct
 from array import array
+from itertools import accumulate
 
 from . import hip
 
@@ -199,22 +200,18 @@ class AdamW:
 
         L = hip.lib()
         chunk, most = L.netop_adamw_chunk(), L.netop_adamw_max_grads()
-        n = torch.tensor(ns, dtype=torch.int64)
-        count = (n + chunk - 1) // chunk
-        of = torch.repeat_interleave(torch.arange(len(ns)), count)
-        start = (torch.arange(len(of)) - (torch.cumsum(count, 0) - count)[of]) * chunk
-        table = torch.empty(len(of), 4, dtype=torch.int64)
-        table[:, 0] = torch.tensor(self._ptrs)[of] + start * self.params[0].element_size()
-        table[:, 1] = torch.tensor(self.offsets)[of] + start
-        table[:, 2] = start
-        table[:, 3] = torch.minimum(n[of] - start, torch.tensor(chunk)) | (of % most) << 32
-        self._table = table.to(self.device)
-        self._launches = []  # (first tensor, one behind the last, address of its chunks, how many)
-        at = 0
-        for a in range(0, len(ns), most):
-            c = int(count[a:a + most].sum())
-            self._launches.append((a, min(a + most, len(ns)), self._table.data_ptr() + at * 32, c))
-            at += c
+        counts = [-(-n // chunk) for n in ns]
+        # a row a tensor: its address, place in the states, elements, first chunk, chunks
+        firsts = [0, *accumulate(counts)]
+        rows = torch.tensor([self._ptrs, self.offsets, ns, firsts[:-1], counts], device=self.device)
+        of = torch.repeat_interleave(torch.arange(len(ns), device=self.device), rows[4], output_size=firsts[-1])
+        start = (torch.arange(firsts[-1], device=self.device) - rows[3][of]) * chunk
+        self._table = torch.stack([rows[0][of] + start * self.params[0].element_size(), rows[1][of] + start, start,
+                                   (rows[2][of] - start).clamp(max=chunk) | (of % most) << 32], 1)
+        # (first tensor, one behind the last, address of its chunks, how many)
+        at = self._table.data_ptr()
+        self._launches = [(a, b, at + 32 * firsts[a], firsts[b] - firsts[a])
+                          for a in range(0, len(ns), most) for b in (min(a + most, len(ns)),)]
 
     def state_dict(self) -> dict:
         """The states themselves (not copies); ``None`` for those this optimizer has not."""

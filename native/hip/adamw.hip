@@ -224,7 +224,7 @@ __global__ __launch_bounds__(kThreads) void adamw_kernel(StepParams a, Grads gra
 // 1 - b^step cancels.
 __global__ void hyper_kernel(Hyper* out, Hyper h, double b1, double b2, double lr, double decay, uint32_t seed,
                              const float* lr_dev, const int64_t* step_dev, int64_t step) {
-    if (step_dev) step = *step_dev;
+    if (step_dev) step = *step_dev < 1 ? 1 : *step_dev;
     if (lr_dev) lr = double(*lr_dev);
     h.alpha = float(lr / -expm1(double(step) * log(b1)));
     h.rc2 = float(1.0 / sqrt(-expm1(double(step) * log(b2))));
@@ -299,10 +299,12 @@ __global__ __launch_bounds__(kThreads) void sumsq_kernel(NormGroup group, NormAr
 #pragma unroll
             for (int j = 0; j < 8; ++j) s = fma(double(float(v[u][j])), double(float(v[u][j])), s);
     }
-    for (; i < n; i += kStep) {
-        const int m = n - i < 8 ? int(n - i) : 8;
-        for (int j = 0; j < m; ++j) s = fma(double(float(p[i + j])), double(float(p[i + j])), s);
+    for (; i + 8 <= n; i += kStep) {
+        const Vec<G, 8> v = Wide<G, 8>::load(p + i);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) s = fma(double(float(v[j])), double(float(v[j])), s);
     }
+    for (; i < n; ++i) s = fma(double(float(p[i])), double(float(p[i])), s);  // one thread's last elements
     s = lanes_sum<64>(s);
     if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
     __syncthreads();
@@ -344,11 +346,13 @@ __global__ __launch_bounds__(kFinalThreads) void sumsq_final_kernel(NormGroup gr
     }
 }
 
+constexpr int kOverlap = -1;  // ops/adamw.py raises ValueError for it
+
 }  // namespace
 
 extern "C" {
 
-// Returns hipError_t values (0 = success).
+// Return hipError_t values (0 = success).
 
 int netop_adamw_chunk() { return kChunk; }
 int netop_adamw_max_grads() { return kMaxGrads; }
@@ -361,7 +365,8 @@ int netop_adamw_step(const StepParams* p, const void* const* grads, hipStream_t 
         (p->ptype != kF32 && !p->master))
         return int(hipErrorInvalidValue);
     if (p->n_chunks == 0) return int(hipSuccess);
-    if (!p->chunks) return int(hipErrorInvalidValue);
+    // A grid's threads are counted in 32 bits.
+    if (!p->chunks || uint64_t(p->n_chunks) * kThreads > 0xffffffffu) return int(hipErrorInvalidValue);
     const OnDevice on(p->device);
     if (on.err != hipSuccess) return int(on.err);
     Grads g;
@@ -395,12 +400,25 @@ int netop_grad_norm(const void* const* grads, const uint64_t* n, int tensors, in
                     hipStream_t stream) {
     if (!grads || !n || tensors < 1 || !workspace || !total || stretch < 1 || dtype < kF32 || dtype > kF16)
         return int(hipErrorInvalidValue);
+    const struct {
+        const void* at;
+        uint64_t n;
+    } outs[3] = {{total, 4}, {coef, 4}, {norms, uint64_t(tensors) * 4}};
+    const auto meet = [](const void* a, uint64_t n, const void* b, uint64_t m) {
+        const auto x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+        return x && y && n && m && x < y + m && y < x + n;
+    };
+    for (int i = 0; i < 3; ++i)
+        for (int j = 0; j < i; ++j)
+            if (meet(outs[i].at, outs[i].n, outs[j].at, outs[j].n)) return kOverlap;
     uint64_t need = 0;
     for (int i = 0; i < tensors; ++i) {
         if (n[i] && !grads[i]) return int(hipErrorInvalidValue);
         need += (n[i] + stretch - 1) / stretch;
+        for (const auto& o : outs)  // a later group's gradients are read after this one's norms are written
+            if (meet(o.at, o.n, grads[i], n[i] * (dtype == kF32 ? 4 : 2))) return kOverlap;
     }
-    if (need > stretches || need > 0x7fffffffu) return int(hipErrorInvalidValue);
+    if (need > stretches || need * kThreads > 0xffffffffu) return int(hipErrorInvalidValue);
     const OnDevice on(device);
     if (on.err != hipSuccess) return int(on.err);
     NormArgs a{};

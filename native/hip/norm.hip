@@ -23,6 +23,7 @@ namespace {
 constexpr int kMaxIn = 9;         // eight partial sums and the residual
 constexpr int kMaxCols = 32768;   // a row in the registers of one workgroup
 constexpr int kGroup = 128;       // columns that share a scale
+constexpr uint64_t kMaxRows = 1 << 21;  // of a launch: rows x 1024 threads stay below 2^32, the most a grid may have
 
 enum Out : int { kSame = 0, kRowScale = 1, kGroupScale = 2 };
 
@@ -625,13 +626,27 @@ int netop_add_rms_norm(const NormParams* p, hipStream_t stream) {
     }
     const OnDevice on(p->device);
     if (on.err != hipSuccess) return int(on.err);
-    switch (p->dtype) {
-        case kF32: norm_of<float>(*p, stream); break;
-        case kBf16: norm_of<__bf16>(*p, stream); break;
-        case kF16: norm_of<_Float16>(*p, stream); break;
-        default: return int(hipErrorInvalidValue);
+    const auto moved = [](auto* q, int64_t bytes) { return q ? static_cast<decltype(q)>(static_cast<void*>(
+        const_cast<char*>(static_cast<const char*>(static_cast<const void*>(q))) + bytes)) : q; };
+    for (uint64_t r = 0; r < rows; r += kMaxRows) {
+        NormParams a = *p;
+        const int64_t at = int64_t(r);
+        a.rows = rows - r < kMaxRows ? rows - r : kMaxRows;
+        for (int k = 0; k < a.n_in; ++k) a.in[k] = moved(a.in[k], at * a.in_stride[k] * int64_t(es));
+        a.out = moved(a.out, at * a.out_stride * (a.out_kind == kSame ? int64_t(es) : 1));
+        a.h = moved(a.h, at * a.h_stride * int64_t(es));
+        a.rstd = moved(a.rstd, at * 4);
+        a.scales = moved(a.scales, at * int64_t(groups) * 4);
+        switch (a.dtype) {
+            case kF32: norm_of<float>(a, stream); break;
+            case kBf16: norm_of<__bf16>(a, stream); break;
+            case kF16: norm_of<_Float16>(a, stream); break;
+            default: return int(hipErrorInvalidValue);
+        }
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return int(e);
     }
-    return int(hipGetLastError());
+    return int(hipSuccess);
 }
 
 // How many rows of `cols` floats the backward pass needs as workspace.

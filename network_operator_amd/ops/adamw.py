@@ -21,6 +21,7 @@ import math
 import struct
 from array import array
 from itertools import accumulate
+from operator import attrgetter
 
 from . import hip
 
@@ -29,6 +30,7 @@ BLOCK = 256  # elements of a tensor that share a scale; every tensor's states st
 # native/hip/adamw.hip:Hyper and StepParams
 _HYPER = struct.Struct("=9fI")
 _STEP = struct.Struct("=8Q" + "9fI" + "6i")
+_OVERLAP = -1
 
 
 def _kinds():
@@ -41,6 +43,31 @@ def _kinds():
 
 
 _KINDS = None
+
+
+_dtype, _shape = attrgetter("dtype"), attrgetter("shape")
+
+
+def _gradients(grads):
+    """The type and device that all ``grads`` but the ``None`` among them share, and their addresses."""
+    import torch
+
+    given = [g for g in grads if g is not None]
+    if not given:
+        return None, -1, [0] * len(grads)
+    dtype, device = given[0].dtype, given[0].get_device()
+    if dtype not in (_KINDS or _kinds()):
+        raise ValueError(f"gradients: expected fp32, bf16 or fp16, got {dtype}")
+    for other in set(map(_dtype, given)):
+        if other is not dtype:
+            raise ValueError(f"gradients must have one type: {dtype} and {other}")
+    if not all(map(torch.Tensor.is_contiguous, given)):
+        raise ValueError("gradients must be contiguous")
+    if device < 0 or len(set(map(torch.Tensor.get_device, given))) > 1:
+        raise ValueError("every tensor must be on one CUDA device")
+    if len(given) == len(grads):
+        return dtype, device, list(map(torch.Tensor.data_ptr, grads))
+    return dtype, device, [0 if g is None else g.data_ptr() for g in grads]
 
 
 def _one(t, dtype, device, what):
@@ -65,54 +92,38 @@ def grad_norm(grads, total, *, norms=None, coef=None, max_norm=None, scale=1.0) 
     """
     import torch
 
-    kinds = _KINDS or _kinds()
-    first = next((g for g in grads if g is not None), None)
-    if first is None:
-        raise ValueError("no gradients")
-    dtype, device = first.dtype, first.get_device()
-    if dtype not in kinds:
-        raise ValueError(f"gradients: expected fp32, bf16 or fp16, got {dtype}")
     limit = math.inf if max_norm is None else float(max_norm)
     if not limit >= 0:
         raise ValueError("max_norm must not be negative")
-    if not math.isfinite(scale):
-        raise ValueError("scale must be finite")
-    ptrs, ns = [], []
-    for g in grads:
-        if g is None:
-            ptrs.append(0)
-            ns.append(0)
-            continue
-        if g.dtype is not dtype:
-            raise ValueError(f"gradients must have one type: {dtype} and {g.dtype}")
-        if not g.is_contiguous():
-            raise ValueError("gradients must be contiguous")
-        if g.get_device() != device:
+    if not 0 <= scale < math.inf:
+        raise ValueError("scale must be finite and not negative")
+    for t, what in ((total, "total"), (coef, "coef")):
+        if t is not None and (t.dtype != torch.float32 or t.numel() != 1):
+            raise ValueError(f"{what}: expected one {torch.float32} element")
+    if norms is not None and (norms.dtype != torch.float32 or norms.shape != (len(grads),) or not norms.is_contiguous()):
+        raise ValueError(f"norms: expected {len(grads)} contiguous float32 elements")
+    dtype, device, ptrs = _gradients(grads)
+    if dtype is None:
+        raise ValueError("no gradients")
+    for t in (total, coef, norms):
+        if t is not None and t.get_device() != device:
             raise ValueError("every tensor must be on one CUDA device")
-        ptrs.append(g.data_ptr())
-        ns.append(g.numel())
-    total_ptr = _one(total, torch.float32, device, "total")
-    coef_ptr = 0 if coef is None else _one(coef, torch.float32, device, "coef")
-    norms_ptr = 0
-    if norms is not None:
-        if norms.dtype != torch.float32 or norms.shape != (len(ns),) or not norms.is_contiguous():
-            raise ValueError(f"norms: expected {len(ns)} contiguous float32 elements")
-        if norms.get_device() != device:
-            raise ValueError("every tensor must be on one CUDA device")
-        norms_ptr = norms.data_ptr()
-    if device < 0:
-        raise ValueError("every tensor must be on one CUDA device")
+    ns = [0 if g is None else g.numel() for g in grads]
     elements = sum(ns)
     stretch = 1 << 13  # elements a workgroup: enough of them to fill the chip, few enough to add up
     while stretch < 1 << 16 and elements // stretch > 4096:
         stretch *= 2
     stretches = elements // stretch + len(ns)
-    work = torch.empty(stretches + len(ns), dtype=torch.float64, device=first.device)
+    work = torch.empty(stretches + len(ns), dtype=torch.float64, device=total.device)
     table = array("Q", ptrs + ns)
     at = table.buffer_info()[0]
-    hip._check((hip._lib or hip.lib()).netop_grad_norm(at, at + 8 * len(ns), len(ns), kinds[dtype], stretch,
-                                                       work.data_ptr(), stretches, total_ptr, norms_ptr, coef_ptr,
-                                                       scale, limit, device, hip._raw_stream(device)), "netop_grad_norm")
+    rc = (hip._lib or hip.lib()).netop_grad_norm(
+        at, at + 8 * len(ns), len(ns), _KINDS[dtype], stretch, work.data_ptr(), stretches, total.data_ptr(),
+        0 if norms is None else norms.data_ptr(), 0 if coef is None else coef.data_ptr(), scale, limit, device,
+        hip._raw_stream(device))
+    if rc == _OVERLAP:
+        raise ValueError("total, norms and coef must not share memory with each other or a gradient")
+    hip._check(rc, "netop_grad_norm")
 
 
 class AdamW:
@@ -233,9 +244,11 @@ class AdamW:
 
     def step(self, grads, *, step, lr=None, coef=None, scale=1.0) -> None:
         """One step from ``grads``, one a parameter: contiguous, of its shape, all of one type (fp32,
-        bf16 or fp16).  A parameter whose gradient is ``None`` is left as it is, with its states.
+        bf16 or fp16).  A parameter whose gradient is ``None`` is left as it is, with its states.  A
+        gradient may be its own parameter's memory, but no other tensor's of this optimizer.
 
-        ``step`` counts from 1: a number, or an int64 tensor of one element on the device.  ``lr``
+        ``step`` counts from 1: a number, or an int64 tensor of one element on the device (one below
+        1 is taken for 1 there).  ``lr``
         replaces the constructor's: a number, or an fp32 tensor of one element.  ``coef`` (an fp32
         tensor of one element, from :func:`grad_norm`) and the number ``scale`` multiply the
         gradients; where the product with ``coef`` is not finite, nothing is changed.
@@ -244,29 +257,17 @@ class AdamW:
 
         if len(grads) != len(self.params):
             raise ValueError(f"{len(self.params)} gradients expected, got {len(grads)}")
-        if [p.data_ptr() for p in self.params] != self._ptrs:
+        if list(map(torch.Tensor.data_ptr, self.params)) != self._ptrs:
             raise ValueError("a parameter has moved since the optimizer was made")
-        device, gtype, ptrs = self._index, None, []
-        for g, shape in zip(grads, self._shapes):
-            if g is None:
-                ptrs.append(0)
-                continue
-            if gtype is None:
-                gtype = g.dtype
-            if g.dtype is not gtype:
-                raise ValueError(f"gradients must have one type: {gtype} and {g.dtype}")
-            if g.shape != shape:
-                raise ValueError(f"a gradient of shape {tuple(g.shape)} for a parameter of shape {tuple(shape)}")
-            if not g.is_contiguous():
-                raise ValueError("gradients must be contiguous")
-            if g.get_device() != device:
-                raise ValueError("every tensor must be on one CUDA device")
-            ptrs.append(g.data_ptr())
+        gtype, device, ptrs = _gradients(grads)
         if gtype is None:
             return
-        kinds = _KINDS or _kinds()
-        if gtype not in kinds:
-            raise ValueError(f"gradients: expected fp32, bf16 or fp16, got {gtype}")
+        if 0 in ptrs or list(map(_shape, grads)) != self._shapes:  # none given, or empty
+            for g, shape in zip(grads, self._shapes):
+                if g is not None and g.shape != shape:
+                    raise ValueError(f"a gradient of shape {tuple(g.shape)} for a parameter of shape {tuple(shape)}")
+        if device != self._index:
+            raise ValueError("every tensor must be on one CUDA device")
         if not math.isfinite(scale):
             raise ValueError("scale must be finite")
         coef_ptr = 0 if coef is None else _one(coef, torch.float32, device, "coef")
@@ -297,5 +298,5 @@ class AdamW:
             block = _STEP.pack(chunks, 0 if self.master is None else self.master.data_ptr(), self.exp_avg.data_ptr(),
                                self.exp_avg_sq.data_ptr(), self.exp_avg_scale.data_ptr() if eight else 0,
                                self.exp_avg_sq_scale.data_ptr() if eight else 0, coef_ptr, on_device, *hyper, n,
-                               self._kind, kinds[gtype], self.state_bits, b - a, device)
+                               self._kind, _KINDS[gtype], self.state_bits, b - a, device)
             hip._check(L.netop_adamw_step(block, at + 8 * a, stream), "netop_adamw_step")

@@ -133,7 +133,9 @@ def _arguments(srcs, weight, out, residual, residual_out, rstd, scales, eps):
         raise ValueError("scales belong to an e4m3 output")
     out_pitch = _pitch(out, shape, e4m3 if kind else dtype, "out", True)
     tensors = [*srcs, weight]
-    pitches = [_pitch(t, shape, dtype, "partial sum") for t in srcs]
+    first, strides = _pitch(srcs[0], shape, dtype, "partial sum"), srcs[0].stride()
+    pitches = [first if t.dtype is dtype and t.shape == shape and t.stride() == strides else
+               _pitch(t, shape, dtype, "partial sum") for t in srcs]  # most are alike
     ptrs = [t.data_ptr() for t in srcs]
     if residual is not None:
         pitches.append(_pitch(residual, shape, dtype, "residual"))

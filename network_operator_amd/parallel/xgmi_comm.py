@@ -238,6 +238,10 @@ class XgmiAllReduce:
         if algo != "one_shot":
             algo = choose_algo(numel, self.world, algo)
         mine = self.input(numel).view(out.shape)
+        held = self.inp.untyped_storage().data_ptr()
+        for t in (out, residual_out, rstd, scales):
+            if t is not None and t.untyped_storage().data_ptr() == held:
+                raise ValueError("an output in the symmetric input buffer: the peers may still be reading it")
         one_shot = algo == "one_shot" or self.world == 1
         args = N._arguments([mine] * (self.world if one_shot else 1), weight, out, residual, residual_out, rstd, scales, eps)
         if args is None:

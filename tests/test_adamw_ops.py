@@ -474,6 +474,17 @@ def test_grad_norm_of_extremes(cuda_device):
     assert math.isnan(t) and math.isnan(c)
 
 
+@pytest.mark.gpu
+def test_grad_norm_refuses_outputs_that_share_memory(cuda_device):
+    b = torch.ones(64, device=cuda_device)
+    for total, kw in [(b[:1], dict(coef=b[:1])), (b[3:4], dict(norms=b[2:4])), (b[40:41], {}), (b[:1], dict(norms=b[32:34])),
+                      (b[:1], dict(coef=b[63:]))]:
+        with pytest.raises(ValueError, match="share memory"):
+            adamw.grad_norm([b[40:], b[33:36]], total, **kw)
+    adamw.grad_norm([b[40:], b[33:36]], b[:1], norms=b[1:3], coef=b[3:4])
+    assert float(b[0]) == pytest.approx(math.sqrt(27), rel=1e-6) and float(b[3]) == 1.0
+
+
 # ---- together with the norm ---------------------------------------------------------------------
 @pytest.mark.gpu
 def test_a_training_step_of_all_operators(cuda_device):

@@ -50,11 +50,13 @@ def run_norm(rank, world):
         norm.add_rms_norm(parts, w, want[0], residual=res, residual_out=want[1], rstd=want[2], scales=want[3])
         wrong[f"{i} {rows}x{cols} {algo} {kind}"] = sum(
             int((a.view(torch.uint8) != b.view(torch.uint8)).sum()) for a, b in zip(got, want) if a is not None and a.numel())
-    try:
-        comm.all_reduce_norm(w, torch.empty(4, 64, device=DEV))
-        wrong["fp32 accepted"] = 1
-    except ValueError:
-        pass
+    for what, out in (("fp32", torch.empty(4, 64, device=DEV)), ("in the input buffer", comm.input(256).view(4, 64)),
+                      ("too large", torch.empty(1 << 14, 64, dtype=torch.bfloat16, device=DEV))):
+        try:
+            comm.all_reduce_norm(w, out)
+            wrong[what + " accepted"] = 1
+        except ValueError:
+            pass
     comm.close()
     return wrong
 

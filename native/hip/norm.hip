@@ -9,11 +9,15 @@
 // The n = 1..8 partial sums may be peer memory (the one-shot all-reduce of xgmi_comm.py reads
 // every rank's partials in place), so no sum is written before it is normalised.
 //
-// One workgroup or one wavefront keeps a row of h in registers, so every input is read once and
-// every output written once.  Bound by HBM; the arithmetic is about ten operations an element.
+// A row of h stays in the registers of a workgroup, or of a part of a wavefront, so every input is read
+// once and every output written once.  Bound by HBM, the arithmetic is about ten operations an element:
+// 16384 x 8192 bf16 with a residual to e4m3 takes 170 us (5.5 TB/s, a large copy's rate).  Few rows are bound by
+// the way there and back: 64 x 8192 over 8 partial sums 5.8 us, one row of 4096 2.8 us.
 //
 // Backward, with g = dy weight:  dh = rstd g - h rstd^3 mean(g h) + dresidual, which is the
 // gradient of every partial sum and of the residual alike; dweight = sum over rows of dy h rstd.
+// 8192 x 4096 bf16 takes 43 us and 5 us for dweight (5.5 TB/s); where rows are few and wide, one workgroup a CU
+// and the partial rows of dweight bound it: 333 x 10007 fp32 13 + 5 us, at 7 us of data.
 #include "elem.hpp"
 
 using namespace netop;

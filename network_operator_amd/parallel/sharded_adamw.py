@@ -7,7 +7,7 @@ between them: rank d, which holds chunk d of the summed gradients anyway, update
 parameters with the states of that chunk alone, and the all-gather carries new parameters instead
 of gradients -- the same bytes over the links, 1/n of the optimizer's memory and work on each GPU.
 
-    comm = XgmiAllReduce(capacity_bytes=2 * sum(p.numel() for p in params) + 4096)
+    comm = XgmiAllReduce(capacity_bytes=2 * sum(p.numel() + 8 for p in params) + 4096)
     opt = ShardedAdamW(comm, params, lr=3e-4, weight_decay=0.1, state_bits=8, max_norm=1.0)
     for step in range(1, steps + 1):
         loss(...).backward()

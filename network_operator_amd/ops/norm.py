@@ -102,7 +102,8 @@ def add_rms_norm(srcs, weight, out, *, residual=None, residual_out=None, rstd=No
     rounded to nearest even; ``code * scale`` is the value.
 
     Sums and statistics are fp32; ``out`` comes from the unrounded sum and is rounded once.  An
-    infinity or NaN in a row makes that row (in 8 bits: its scale) NaN or infinite and no other.
+    infinity or NaN in a row makes that row (in 8 bits: its scale) NaN or infinite and no other.  Squares
+    beyond fp32's range, of rows with values from about 1e19 on, make ``rstd`` and ``out`` zero.
     """
     args = _arguments(srcs, weight, out, residual, residual_out, rstd, scales, eps)
     if args:

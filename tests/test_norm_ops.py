@@ -267,6 +267,16 @@ def test_tiny_and_huge_rows(cuda_device):
 
 
 @pytest.mark.gpu
+def test_squares_beyond_fp32_make_a_row_zero_and_no_other(cuda_device):
+    x = torch.randn(3, 600, device=cuda_device)
+    x[1] *= 1e25
+    out, rstd, w = torch.empty_like(x), torch.empty(3, device=cuda_device), torch.rand(600, device=cuda_device)
+    norm.add_rms_norm([x], w, out, rstd=rstd)
+    assert float(rstd[1]) == 0 and bool((out[1] == 0).all())
+    _check([x[::2]], None, w, None, rstd[::2], out[::2])
+
+
+@pytest.mark.gpu
 def test_row_offsets_pass_32_bits(cuda_device):
     pitch = (1 << 31) + 8  # elements; row 2 starts 8 GiB in
     free, _ = torch.cuda.mem_get_info(cuda_device)

@@ -493,11 +493,12 @@ Shape shape_for(int cols, uint64_t rows) {
 
 // Workgroups of the backward pass, each with a partial row of dweight: as many as are at work together, and
 // few where rows are few, since a partial row costs two rows of fp32.  8192 x 4096 bf16: 512 50 us, 256 66,
-// 1024 57; 8192 x 7168 fp32: 256 172 us, 512 182; 1000 x 5003 bf16: 256 17.4 us, 512 21.7.
+// 1024 57; 8192 x 7168 fp32: 256 172 us, 512 182; 1000 x 5003 bf16: 256 17.4 us, 512 21.7; 65536 x 1024 bf16
+// (two rows a workgroup): 768 96 us, 512 109, 1024 99.
 int parts_for(int cols, uint64_t rows) {
     const Shape s = shape_for(cols, rows);
     const uint64_t at_once = cols < 8 ? 256 : s.tpr ? 256 / s.tpr : 1;
-    const uint64_t most = cols < 8 || s.tpr ? 1024 : rows >= 2048 && s.vpt == 1 && s.block <= 640 ? 512 : 256;
+    const uint64_t most = cols < 8 || s.tpr ? 768 : rows >= 2048 && s.vpt == 1 && s.block <= 640 ? 512 : 256;
     const uint64_t need = (rows + at_once - 1) / at_once, turns = (need + most - 1) / most;
     return turns ? int((need + turns - 1) / turns) : 0;  // all of them as many turns: 333 rows are 167 times two
 }

@@ -233,7 +233,7 @@ __global__ __launch_bounds__(Threads<TPR>::kBlock) void norm_kernel(NormParams a
                 amax = lanes_max<(TPR == 8 ? 8 : 16), true>(amax);
                 if ((t & 15) == 0 && at.in) a.scales[row * groups + (k * n + t) / 16] = amax < kTiny ? 0.0f : amax / kE4m3Max;
             }
-            const float inv = amax < kTiny ? 0.0f : kE4m3Max / amax;
+            const float inv = amax < kTiny ? 0.0f : 1.0f / (amax / kE4m3Max);  // of the scale as it is stored
             if (!at.in) continue;
             Vec<float, 8> q;
 #pragma unroll
@@ -278,7 +278,7 @@ __global__ __launch_bounds__(256) void narrow_norm_kernel(NormParams a) {
             y[c] = h[c] * rstd * (a.weight_f32 ? static_cast<const float*>(a.weight)[c] : float(static_cast<const T*>(a.weight)[c]));
             amax = larger(amax, fabsf(y[c]));
         }
-    const float inv = amax < kTiny ? 0.0f : kE4m3Max / amax;
+    const float inv = amax < kTiny ? 0.0f : 1.0f / (amax / kE4m3Max);  // of the scale as it is stored
     if (a.out_kind != kSame) a.scales[row] = amax < kTiny ? 0.0f : amax / kE4m3Max;
 #pragma unroll
     for (int c = 0; c < 7; ++c)

@@ -98,8 +98,9 @@ def add_rms_norm(srcs, weight, out, *, residual=None, residual_out=None, rstd=No
 
     ``out`` has the inputs' type, or is ``float8_e4m3fn`` with ``scales`` (fp32): of shape ``(...)``
     for one scale a row, or ``(..., ceil(cols / 128))`` for one a group of 128 columns.  A scale is
-    the largest magnitude / 448 (zero, with all codes zero, where that is below 2**-100); codes are
-    rounded to nearest even; ``code * scale`` is the value.
+    the largest magnitude / 448 (zero, with all codes zero, where the magnitude is below 2**-100); a code
+    is the value times the scale's reciprocal, both in fp32, rounded to nearest even; ``code * scale`` is
+    the value.
 
     Sums and statistics are fp32; ``out`` comes from the unrounded sum and is rounded once.  An
     infinity or NaN in a row makes that row (in 8 bits: its scale) NaN or infinite and no other.  Squares

@@ -14,8 +14,9 @@
 // 16384 x 8192 bf16 with a residual to e4m3 takes 170 us (5.5 TB/s, a large copy's rate).  Few rows are bound by
 // the way there and back: 64 x 8192 over 8 partial sums 5.8 us, one row of 4096 2.8 us.
 //
-// Backward, with g = dy weight:  dh = rstd g - h rstd^3 mean(g h) + dresidual, which is the
-// gradient of every partial sum and of the residual alike; dweight = sum over rows of dy h rstd.
+// Backward, with x = h rstd and g = dy weight:  dh = rstd (g - x mean(g x)) + dresidual, which is the
+// gradient of every partial sum and of the residual alike; dweight = sum over rows of dy x.  x is of
+// order one whatever h is; rstd^3 would leave fp32 for rows of 1e13 or 1e-13, and dy h for others.
 // 8192 x 4096 bf16 takes 43 us and 5 us for dweight (5.5 TB/s); where rows are few and wide, one workgroup a CU
 // and the partial rows of dweight bound it: 333 x 10007 fp32 13 + 5 us, at 7 us of data.
 #include "elem.hpp"
@@ -337,14 +338,14 @@ __global__ __launch_bounds__(Threads<TPR>::kBlock) void norm_backward_kernel(Nor
                     raw_h.v[k] = Wide<T, 8>::load(hp + at.c);
                 }
                 if constexpr (!kWeights) weight[k] = weights8<T>(a.weight, a.weight_f32, at.c);
-                const Vec<float, 8> g = widen<T, 8>(raw_g.v[k]), h = widen<T, 8>(raw_h.v[k]);
-                dw[k] += g * h * rstd;
-                dot = dot8(g * weight[k], h, at.twice, dot);
+                const Vec<float, 8> g = widen<T, 8>(raw_g.v[k]), x = widen<T, 8>(raw_h.v[k]) * rstd;
+                dw[k] += g * x;
+                dot = dot8(g * weight[k], x, at.twice, dot);
             }
             if constexpr (!kWeights) asm volatile("" ::: "memory");  // holds back the next vector's loads
         }
         dot = row_sum<TPR>(dot, red[turn]);
-        const float back = rstd * rstd * rstd * (dot / float(a.cols));
+        const float back = dot / float(a.cols);
         Vec<T, 8> d[VPT];
 #pragma unroll
         for (int k = 0; k < VPT; ++k) {
@@ -356,9 +357,10 @@ __global__ __launch_bounds__(Threads<TPR>::kBlock) void norm_backward_kernel(Nor
                     if (rp) raw_r.v[k] = Wide<T, 8>::load(rp + at.c);
                 }
                 if constexpr (!kWeights) weight[k] = weights8<T>(a.weight, a.weight_f32, at.c);
-                Vec<float, 8> x = rstd * (widen<T, 8>(raw_g.v[k]) * weight[k]) - widen<T, 8>(raw_h.v[k]) * back;
-                if (rp) x += widen<T, 8>(raw_r.v[k]);
-                d[k] = narrow<T, 8>(x);
+                const Vec<float, 8> x = widen<T, 8>(raw_h.v[k]) * rstd;
+                Vec<float, 8> y = rstd * (widen<T, 8>(raw_g.v[k]) * weight[k] - x * back);
+                if (rp) y += widen<T, 8>(raw_r.v[k]);
+                d[k] = narrow<T, 8>(y);
                 if constexpr (!kTwice) Wide<T, 8>::store(dh + at.c, d[k]);
             }
             if constexpr (!kWeights) asm volatile("" ::: "memory");
@@ -402,22 +404,22 @@ __global__ __launch_bounds__(256) void narrow_backward_kernel(NormBackwardParams
         const T* rp = a.dres ? static_cast<const T*>(a.dres) + int64_t(row) * a.dres_stride : nullptr;
         T* dh = static_cast<T*>(a.dh) + int64_t(row) * a.dh_stride;
         const float rstd = a.rstd[row];
-        float g[7], h[7], dot = 0;
+        float g[7], x[7], dot = 0;
 #pragma unroll
         for (int c = 0; c < 7; ++c) {
-            g[c] = h[c] = 0;
+            g[c] = x[c] = 0;
             if (c < a.cols) {
                 g[c] = float(dy[c]);
-                h[c] = float(hp[c]);
+                x[c] = float(hp[c]) * rstd;
             }
-            dw[c] += g[c] * h[c] * rstd;
+            dw[c] += g[c] * x[c];
             g[c] *= w[c];
-            dot = fmaf(g[c], h[c], dot);
+            dot = fmaf(g[c], x[c], dot);
         }
-        const float back = rstd * rstd * rstd * (dot / float(a.cols));
+        const float back = dot / float(a.cols);
 #pragma unroll
         for (int c = 0; c < 7; ++c)
-            if (c < a.cols) dh[c] = T(rstd * g[c] - h[c] * back + (rp ? float(rp[c]) : 0.0f));
+            if (c < a.cols) dh[c] = T(rstd * (g[c] - x[c] * back) + (rp ? float(rp[c]) : 0.0f));
     }
 #pragma unroll
     for (int c = 0; c < 7; ++c) {

@@ -103,8 +103,10 @@ def add_rms_norm(srcs, weight, out, *, residual=None, residual_out=None, rstd=No
     the value.
 
     Sums and statistics are fp32; ``out`` comes from the unrounded sum and is rounded once.  An
-    infinity or NaN in a row makes that row (in 8 bits: its scale) NaN or infinite and no other.  Squares
-    beyond fp32's range, of rows with values from about 1e19 on, make ``rstd`` and ``out`` zero.
+    infinity or NaN in a row makes that row (in 8 bits: its scale) NaN or infinite and no other.  A row
+    whose squares add up to more than fp32 holds (a root mean square of 1.8e19 / sqrt(cols)) has ``rstd``
+    and ``out`` zero.  With ``eps`` zero, squares below 1e-38 lose their precision (a root mean square of
+    1e-19), and a row of zeros is NaN.
     """
     args = _arguments(srcs, weight, out, residual, residual_out, rstd, scales, eps)
     if args:
@@ -179,7 +181,8 @@ def add_rms_norm_backward(dy, h, weight, rstd, dh, dweight, *, dresidual=None) -
     ``h`` is its ``residual_out`` and ``rstd`` its ``rstd``; ``dy`` the gradient of ``out``,
     ``dresidual``, where given, that of ``residual_out``.  ``dh`` takes the gradient of the sum, which
     is that of each partial sum and of the residual (for one that was a row for all: its rows' sum),
-    and may be ``dy``, ``h`` or ``dresidual`` itself.  ``dweight`` (``(cols,)``, the weight's type or
+    and may be ``dy``, ``h`` or ``dresidual`` itself.  It is right for rows of any magnitude that the forward
+    pass takes; where ``rstd`` is zero it is ``dresidual``.  ``dweight`` (``(cols,)``, the weight's type or
     fp32) takes the weight's gradient, summed over the rows in fp32 in an order that depends on the
     shape alone: the same inputs give the same bits.
     """

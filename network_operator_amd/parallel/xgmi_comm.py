@@ -229,7 +229,8 @@ class XgmiAllReduce:
 
         ``one_shot`` reads the peers' partial sums in the norm kernel, and the sum is never rounded
         before it is normalised; it takes any number of elements.  The two-shot variants (see
-        :func:`choose_algo`) normalise :meth:`all_reduce`'s result, which is rounded to bf16 once."""
+        :func:`choose_algo`) normalise :meth:`all_reduce`'s result, which is rounded to bf16 once; they write
+        :meth:`output`, and a ``residual`` or ``weight`` that lies there is copied first."""
         import torch
 
         numel = out.numel()
@@ -243,6 +244,14 @@ class XgmiAllReduce:
             if t is not None and t.untyped_storage().data_ptr() == held:
                 raise ValueError("an output in the symmetric input buffer: the peers may still be reading it")
         one_shot = algo == "one_shot" or self.world == 1
+        if not one_shot:
+            # The sum goes into the output buffer, where views of earlier results may serve as inputs here.
+            start = self.out.data_ptr()
+
+            def kept(t):
+                return t.clone() if t is not None and start <= t.data_ptr() < start + numel * 2 else t
+
+            residual, weight = kept(residual), kept(weight)
         args = N._arguments([mine] * (self.world if one_shot else 1), weight, out, residual, residual_out, rstd, scales, eps)
         if args is None:
             return

@@ -1,0 +1,77 @@
+"""Rank process of tests/test_xgmi_ops_buffers.py: where the operators' tensors lie in the symmetric
+buffers; all ranks on GPU 0.
+
+    RANK=r WORLD_SIZE=n NETOP_INIT_FILE=... python xgmi_ops_buffers_worker.py MODE [ARGUMENT]
+"""
+
+import faulthandler
+import json
+import os
+import sys
+
+import torch
+import torch.distributed as dist
+
+from network_operator_amd.ops import norm
+from network_operator_amd.parallel.xgmi_comm import XgmiAllReduce
+
+faulthandler.dump_traceback_later(float(os.environ.get("NETOP_RANK_HANG_S", "90")), exit=True)
+DEV = torch.device("cuda", 0)
+
+
+def _bf16(shape, seed, scale=1.0):
+    g = torch.Generator().manual_seed(seed)
+    return (torch.randn(shape, generator=g) * scale).bfloat16().to(DEV)
+
+
+def _differ(a, b):
+    return a.shape != b.shape or int((a.contiguous().view(torch.uint8) != b.contiguous().view(torch.uint8)).sum())
+
+
+def run_residual(rank, world):
+    """A residual or weight in the output buffer, which the two-shot variants write: the norm is that of
+    the values it had.  On every rank, or on one alone."""
+    rows, cols = 2112, 1024  # 4.1 MiB: "auto" takes two shots
+    n = rows * cols
+    comm = XgmiAllReduce(16 << 20, device=DEV)
+    w = (1 + 0.1 * _bf16(cols, 1).float()).bfloat16()
+    wrong = {}
+    for i, (algo, where) in enumerate([("two_shot", "residual"), ("two_shot_push", "residual"), ("auto", "residual"),
+                                       ("one_shot", "residual"), ("two_shot", "rank 0"), ("two_shot", "in place"),
+                                       ("two_shot", "weight"), ("two_shot", "behind the message")]):
+        parts = [_bf16((rows, cols), 100 * i + r, 0.5) for r in range(world)]
+        res = _bf16((rows, cols), 100 * i + 99)
+        out, want, h, want_h = (torch.empty(rows, cols, dtype=torch.bfloat16, device=DEV) for _ in range(4))
+        residual, weight = res, w
+        if where == "weight":
+            weight = comm.output(cols)
+            weight.copy_(w)
+        elif where == "behind the message":
+            residual = comm.output(2 * n)[n:].view(rows, cols)
+            residual.copy_(res)
+        elif where != "rank 0" or rank == 0:
+            residual = comm.output(n).view(rows, cols)
+            residual.copy_(res)
+            h = residual if where == "in place" else h
+        comm.input(n).view(rows, cols).copy_(parts[rank])
+        comm.all_reduce_norm(weight, out, residual=residual, residual_out=h, algo=algo)
+        total = torch.zeros(rows, cols, device=DEV)
+        for p in parts:
+            total += p.float()
+        norm.add_rms_norm(parts if algo == "one_shot" or world == 1 else [total.bfloat16()], w, want, residual=res,
+                          residual_out=want_h)
+        wrong[f"{algo} {where}"] = _differ(out, want) + _differ(h, want_h)
+    comm.close()
+    return wrong
+
+
+def main():
+    rank, world = int(os.environ["RANK"]), int(os.environ["WORLD_SIZE"])
+    dist.init_process_group("gloo", init_method=f"file://{os.environ['NETOP_INIT_FILE']}", rank=rank, world_size=world)
+    torch.cuda.set_device(DEV)
+    print("RESULT " + json.dumps(globals()["run_" + sys.argv[1]](rank, world, *sys.argv[2:])), flush=True)
+    dist.destroy_process_group()
+
+
+if __name__ == "__main__":
+    main()

@@ -263,8 +263,10 @@ class XgmiAllReduce:
         args[0][:self.world] = self.peer_in  # in rank order, this rank's among them
         stream = torch.cuda.current_stream(self.device)
         self._sync_and_wait(stream)  # every partial sum is complete
-        N._launch(*args)
-        self._sync_and_wait(stream)  # nobody reads my partial sum any more
+        try:
+            N._launch(*args)
+        finally:  # also of a call that is refused: the peers wait here, and would take the next call's barrier for it
+            self._sync_and_wait(stream)  # nobody reads my partial sum any more
 
     def reduce_scatter(self, numel: int, offset: int = 0):
         """Rank d gets chunk d of the sum of every rank's ``input(offset + numel)[offset:]``

@@ -25,3 +25,25 @@ def _ranks(world, *args):
 def test_a_residual_in_the_output_buffer_keeps_its_values(cuda_device, world):
     for r in _ranks(world, "residual"):
         assert len(r) == 8 and not any(r.values()), r
+
+
+def test_a_refused_norm_does_not_leave_its_peers_at_the_barrier(monkeypatch):
+    """A launch that is refused between the two barriers of the one-shot norm: the rank takes part in both."""
+    from network_operator_amd.parallel import xgmi_comm
+
+    comm = object.__new__(xgmi_comm.XgmiAllReduce)
+    comm.rank, comm.world, comm.capacity, comm.device = 0, 2, 1024, torch.device("cpu")
+    comm.inp, comm.out, comm.peer_in = torch.zeros(1024, dtype=torch.uint8), torch.zeros(1024, dtype=torch.uint8), [1, 2]
+    seen = []
+
+    def refuse(*args):
+        seen.append("launch")
+        raise ValueError("an output overlaps another tensor of the call")
+
+    monkeypatch.setattr(comm, "_sync_and_wait", lambda stream: seen.append("barrier"))
+    monkeypatch.setattr(xgmi_comm.N, "_arguments", lambda *args: ([0, 0],))
+    monkeypatch.setattr(xgmi_comm.N, "_launch", refuse)
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda device=None: None)
+    with pytest.raises(ValueError, match="overlaps"):
+        comm.all_reduce_norm(torch.ones(16), torch.zeros(4, 16, dtype=torch.bfloat16), algo="one_shot")
+    assert seen == ["barrier", "launch", "barrier"]

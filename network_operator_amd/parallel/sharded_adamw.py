@@ -28,8 +28,8 @@ class ShardedAdamW:
     """``params``: contiguous bf16 tensors on ``comm``'s device, the same on every rank (the
     constructor takes rank 0's layout for granted and every rank's values for equal).  Gradients are
     averaged over the ranks, in bf16 as they cross the links; masters and states are fp32, or 8-bit
-    states (:class:`~network_operator_amd.ops.adamw.AdamW`, whose options these are).  With
-    ``max_norm`` gradients are clipped by the norm of all of them; a step whose norm is infinite or
+    states (:class:`~network_operator_amd.ops.adamw.AdamW`, whose options these are), whose blocks start
+    where a rank's part of a parameter does.  With ``max_norm`` gradients are clipped by the norm of all of them; a step whose norm is infinite or
     NaN changes nothing on any rank."""
 
     def __init__(self, comm: XgmiAllReduce, params, *, lr, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.01,
@@ -57,10 +57,24 @@ class ShardedAdamW:
         for p, at in zip(self.params, self.offsets):
             flat[at:at + p.numel()].copy_(p.detach().reshape(-1))
         self.shard = flat[self.mine].clone()
+        # What lies here of each parameter is a tensor of the optimizer's: a block that shares a scale never
+        # spans two.  Sizes of gap, part, gap, part ... for _parts; a rank of none has one empty part.
+        self._sizes, end = [], 0
+        for p, at in zip(self.params, self.offsets):
+            a, b = (min(max(x - self.mine.start, 0), self.chunk) for x in (at, at + p.numel()))
+            if a < b:
+                self._sizes += [a - end, b - a]
+                end = b
+        self._sizes = self._sizes or [0, 0]
+        self._sizes.append(self.chunk - end)
         # every rank its own random numbers: the chunks' positions all start at zero
-        self.opt = A.AdamW([self.shard], lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, state_bits=state_bits,
+        self.opt = A.AdamW(self._parts(self.shard), lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, state_bits=state_bits,
                            seed=(seed + 0x9E3779B1 * comm.rank) % (1 << 32))
         self._norm, self._coef = (torch.empty(1, device=comm.device) for _ in range(2))
+
+    def _parts(self, chunk):
+        """This rank's parts of the parameters, out of a chunk."""
+        return list(chunk.split(self._sizes)[1::2])
 
     def state_dict(self) -> dict:
         """This rank's states (:meth:`AdamW.state_dict`); they belong to this rank, world size and order
@@ -102,7 +116,7 @@ class ShardedAdamW:
             x[end:].zero_()
             mine = comm.reduce_scatter(n)
             norm = self._clip(mine)
-            self.opt.step([mine], step=step, lr=lr, coef=self._coef)
+            self.opt.step(self._parts(mine), step=step, lr=lr, coef=self._coef)
             mine.copy_(self.shard)
             full = comm.all_gather_inplace(n)
             for p, at in zip(self.params, self.offsets):

@@ -47,3 +47,11 @@ def test_a_refused_norm_does_not_leave_its_peers_at_the_barrier(monkeypatch):
     with pytest.raises(ValueError, match="overlaps"):
         comm.all_reduce_norm(torch.ones(16), torch.zeros(4, 16, dtype=torch.bfloat16), algo="one_shot")
     assert seen == ["barrier", "launch", "barrier"]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits", [8, 32])
+@pytest.mark.parametrize("world", [1, 3])
+def test_sharded_states_are_those_of_the_parameters_parts(cuda_device, world, bits):
+    for r in _ranks(world, "pieces", str(bits)):
+        assert not any(r.values()), r

@@ -1,5 +1,5 @@
 """Rank process of tests/test_xgmi_ops_buffers.py: where the operators' tensors lie in the symmetric
-buffers; all ranks on GPU 0.
+buffers, and how the sharded optimizer cuts its states; all ranks on GPU 0.
 
     RANK=r WORLD_SIZE=n NETOP_INIT_FILE=... python xgmi_ops_buffers_worker.py MODE [ARGUMENT]
 """
@@ -12,7 +12,8 @@ import sys
 import torch
 import torch.distributed as dist
 
-from network_operator_amd.ops import norm
+from network_operator_amd.ops import adamw, norm
+from network_operator_amd.parallel.sharded_adamw import ShardedAdamW
 from network_operator_amd.parallel.xgmi_comm import XgmiAllReduce
 
 faulthandler.dump_traceback_later(float(os.environ.get("NETOP_RANK_HANG_S", "90")), exit=True)
@@ -62,6 +63,58 @@ def run_residual(rank, world):
                           residual_out=want_h)
         wrong[f"{algo} {where}"] = _differ(out, want) + _differ(h, want_h)
     comm.close()
+    return wrong
+
+
+def _sums(sizes, step, rank, world, params):
+    """This rank's gradients into ``params``; the gradients of all ranks, summed in rank order in fp32 and
+    rounded to bf16 as the reduce-scatter does."""
+    sums = [torch.zeros(s, device=DEV) for s in sizes]
+    for r in range(world):
+        for k, (p, s) in enumerate(zip(params, sizes)):
+            x = _bf16(s, 10000 * step + 100 * k + r, 0.1)
+            sums[k] += x.float()
+            if r == rank:
+                p.grad = x
+    return [t.bfloat16() for t in sums]
+
+
+def run_pieces(rank, world, bits):
+    """The states are those of AdamW over the parts of the parameters that lie in this rank's chunk, each
+    a tensor of its own: bit for bit, three steps.  Small values beside large ones, a rank without any."""
+    wrong = {}
+    for i, sizes in enumerate([[(33, 5), (1000,), (7,), (64, 64), (300,)], [(9,)]]):
+        scale = [0.02, 1.0, 1e-3, 0.02, 1e-3]
+        comm = XgmiAllReduce(1 << 20, device=DEV)
+        params = [torch.nn.Parameter(_bf16(s, k, scale[k])) for k, s in enumerate(sizes)]
+        opt = ShardedAdamW(comm, params, lr=1e-2, weight_decay=0.1, state_bits=int(bits), seed=5)
+        chunk = opt.numel // world
+        lo, hi = rank * chunk, (rank + 1) * chunk
+        cut = [(k, max(at, lo) - at, min(at + p.numel(), hi) - at) for k, (p, at) in enumerate(zip(params, opt.offsets))
+               if max(at, lo) < min(at + p.numel(), hi)]
+
+        def parts(tensors):
+            return [tensors[k].detach().reshape(-1)[a:b] for k, a, b in cut]
+
+        mine = [t.clone() for t in parts(params)]
+        ref = adamw.AdamW(mine, lr=1e-2, weight_decay=0.1, state_bits=int(bits), seed=(5 + 0x9E3779B1 * rank) % (1 << 32)) if cut else None
+        coef = torch.full((1,), 1 / world, device=DEV)
+        for step in (1, 2, 3):
+            sums = _sums(sizes, step, rank, world, params)
+            for t in (sums[-1], params[-1].grad):  # a small gradient beside the others'
+                t.mul_(2.0 ** -12)
+            opt.step(step)
+            if ref:
+                ref.step(parts(sums), step=step, coef=coef)
+        wrong[f"{i} parameters"] = sum(_differ(a, b) for a, b in zip(parts(params), mine))
+        want = ref.state_dict() if ref else {}
+        for k, t in opt.state_dict().items():
+            if k in want and isinstance(t, torch.Tensor):
+                wrong[f"{i} {k}"] = int(_differ(t, want[k]))
+        gathered = [None] * world
+        dist.all_gather_object(gathered, [p.detach().cpu() for p in params])
+        wrong[f"{i} ranks differ"] = sum(_differ(a, b) for other in gathered for a, b in zip(other, gathered[0]))
+        comm.close()
     return wrong
 
 

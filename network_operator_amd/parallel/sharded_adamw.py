@@ -82,7 +82,10 @@ class ShardedAdamW:
         return self.opt.state_dict()
 
     def load_state_dict(self, state: dict) -> None:
+        """Copies :meth:`state_dict`'s states in; the parameters, which the next step sets, are not touched."""
         self.opt.load_state_dict(state)
+        for part, at in zip(self.opt.params, self.opt.offsets):
+            part.copy_(self.opt.master[at:at + part.numel()])
 
     def _clip(self, grads) -> float:
         """``_coef`` for the norm over every rank's chunk, which it returns."""
@@ -117,6 +120,8 @@ class ShardedAdamW:
             mine = comm.reduce_scatter(n)
             norm = self._clip(mine)
             self.opt.step(self._parts(mine), step=step, lr=lr, coef=self._coef)
+            if not math.isfinite(norm):
+                return norm  # the same on every rank: the parameters stay as they are
             mine.copy_(self.shard)
             full = comm.all_gather_inplace(n)
             for p, at in zip(self.params, self.offsets):

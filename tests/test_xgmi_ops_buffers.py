@@ -55,3 +55,10 @@ def test_a_refused_norm_does_not_leave_its_peers_at_the_barrier(monkeypatch):
 def test_sharded_states_are_those_of_the_parameters_parts(cuda_device, world, bits):
     for r in _ranks(world, "pieces", str(bits)):
         assert not any(r.values()), r
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("world", [1, 2])
+def test_an_overflowed_step_after_loading_keeps_the_loaded_parameters(cuda_device, world):
+    for r in _ranks(world, "load"):
+        assert not any(r.values()), r

@@ -118,6 +118,40 @@ def run_pieces(rank, world, bits):
     return wrong
 
 
+def run_load(rank, world):
+    """States and parameters loaded into an optimizer that was made from others: a step of an infinite
+    norm leaves the parameters as they are, and the next one goes on from the loaded states."""
+    sizes = [(40, 9), (511,)]
+
+    def made(seed):
+        params = [torch.nn.Parameter(_bf16(s, seed + k)) for k, s in enumerate(sizes)]
+        return params, ShardedAdamW(comm, params, lr=1e-2, weight_decay=0.1)
+
+    comm = XgmiAllReduce(1 << 20, device=DEV)
+    old, a = made(0)
+    for step in (1, 2):
+        _sums(sizes, step, rank, world, old)
+        a.step(step)
+    saved = {k: t.clone() if isinstance(t, torch.Tensor) else t for k, t in a.state_dict().items()}
+    new, b = made(50)
+    with torch.no_grad():
+        for p, q in zip(new, old):
+            p.copy_(q)
+    b.load_state_dict(saved)
+    for p in new:
+        p.grad = torch.zeros_like(p)
+    new[1].grad[0] = float("inf")
+    bad = b.step(3)
+    got = {"norm is finite": int(bad != float("inf")), "kept": sum(_differ(p.detach(), q.detach()) for p, q in zip(new, old))}
+    _sums(sizes, 3, rank, world, old)
+    a.step(3)
+    _sums(sizes, 3, rank, world, new)
+    b.step(3)
+    got["next"] = sum(_differ(p.detach(), q.detach()) for p, q in zip(new, old))
+    comm.close()
+    return got
+
+
 def main():
     rank, world = int(os.environ["RANK"]), int(os.environ["WORLD_SIZE"])
     dist.init_process_group("gloo", init_method=f"file://{os.environ['NETOP_INIT_FILE']}", rank=rank, world_size=world)

@@ -62,3 +62,8 @@ def test_sharded_states_are_those_of_the_parameters_parts(cuda_device, world, bi
 def test_an_overflowed_step_after_loading_keeps_the_loaded_parameters(cuda_device, world):
     for r in _ranks(world, "load"):
         assert not any(r.values()), r
+
+
+@pytest.mark.gpu
+def test_a_device_without_an_index_is_the_current_one(cuda_device):
+    assert _ranks(1, "device") == [{"device": 0}]

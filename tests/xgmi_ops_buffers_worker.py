@@ -152,6 +152,17 @@ def run_load(rank, world):
     return got
 
 
+def run_device(rank, world):
+    """A communicator on "cuda" is one on the current device, and takes that device's parameters."""
+    comm = XgmiAllReduce(1 << 20, device="cuda")
+    params = [torch.nn.Parameter(_bf16((64,), 1))]
+    opt = ShardedAdamW(comm, params, lr=1e-2)
+    params[0].grad = torch.ones_like(params[0])
+    opt.step(1)
+    comm.close()
+    return {"device": int(comm.device != DEV)}
+
+
 def main():
     rank, world = int(os.environ["RANK"]), int(os.environ["WORLD_SIZE"])
     dist.init_process_group("gloo", init_method=f"file://{os.environ['NETOP_INIT_FILE']}", rank=rank, world_size=world)

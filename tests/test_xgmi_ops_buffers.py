@@ -67,3 +67,18 @@ def test_an_overflowed_step_after_loading_keeps_the_loaded_parameters(cuda_devic
 @pytest.mark.gpu
 def test_a_device_without_an_index_is_the_current_one(cuda_device):
     assert _ranks(1, "device") == [{"device": 0}]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("world", [1, 3])
+def test_sharded_steps_are_clipped_averaged_and_decayed(cuda_device, world):
+    """In units of u = 2^-24.  A rank's norm is off by 2 u (the factor 1 / ranks, a rounding), the factor by
+    one more, the other side's by 1: with a rounding a side, gradients x differ by 6 u.  M is the largest |x| so
+    far, c_k = 1 - 0.9^k.  m: d_k <= 0.9 d_(k-1) + 0.1 * 6 + 2 sides * 2 c_k, so d_1..3 = 1, 2.3, 3.8 (of M); v (of
+    M^2): 0.001 * (14 + 4 k) a step, 0.07.  The update, at most 1.73 lr: m's share d_k / c_k / 0.58 = 24, sqrt(v)'s
+    (14 + 12) / 2 + 2 = 15 and 12 roundings on the way, (15 + 12) * 1.73 = 47, in units of lr; 4 u a step of the
+    master's own magnitude.  Three steps: 3 * (4 + 24 + 47), with lr added to the magnitude."""
+    rows = _ranks(world, "clip")
+    for r in rows:
+        assert r["exp_avg"] <= 4 and r["exp_avg_sq"] <= 0.1 and r["master"] <= 225 and r["parameters"] == 0, r
+    assert sum(r["checked"] for r in rows) == 33 * 5 + 1000 + 7 + 64 * 64, rows

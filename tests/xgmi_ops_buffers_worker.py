@@ -118,6 +118,42 @@ def run_pieces(rank, world, bits):
     return wrong
 
 
+def run_clip(rank, world):
+    """Clipped and averaged steps against the same steps on whole tensors: masters and moments by how far
+    they are off in units of 2^-24 of what goes into them, parameters by their masters' roundings."""
+    sizes = [(33, 5), (1000,), (7,), (64, 64)]
+    params = [torch.nn.Parameter(_bf16(s, k)) for k, s in enumerate(sizes)]
+    comm = XgmiAllReduce(1 << 20, device=DEV)
+    opt = ShardedAdamW(comm, params, lr=1e-2, weight_decay=0.1, max_norm=0.5)
+    whole = adamw.AdamW([p.detach().clone() for p in params], lr=1e-2, weight_decay=0.1)
+    total, coef = torch.empty(1, device=DEV), torch.empty(1, device=DEV)
+    mags = [torch.zeros(s, device=DEV) for s in sizes]
+    for step in (1, 2, 3):
+        sums = _sums(sizes, step, rank, world, params)
+        opt.step(step)
+        adamw.grad_norm(sums, total, coef=coef, max_norm=0.5, scale=1 / world)
+        whole.step(sums, step=step, coef=coef)
+        for m, s in zip(mags, sums):
+            m.copy_(torch.maximum(m, s.float().abs() * coef))
+    lo, hi = opt.mine.start, opt.mine.stop
+    off, checked = dict(master=0.0, exp_avg=0.0, exp_avg_sq=0.0, parameters=0), 0
+    at = 0  # in this rank's states
+    for k, (p, start) in enumerate(zip(params, opt.offsets)):
+        a, b = max(start, lo), min(start + p.numel(), hi)
+        if a >= b:
+            continue
+        here, there = slice(at, at + b - a), slice(whole.offsets[k] + a - start, whole.offsets[k] + b - start)
+        mag = mags[k].reshape(-1)[a - start:b - start]
+        for name, scale in (("master", whole.master[there].abs() + 0.01), ("exp_avg", mag), ("exp_avg_sq", mag * mag)):
+            x, y = getattr(opt.opt, name)[here], getattr(whole, name)[there]
+            off[name] = max(off[name], float(((x - y).abs() / scale.clamp(min=1e-30)).max()) * 2 ** 24)
+        off["parameters"] += _differ(p.detach().reshape(-1)[a - start:b - start], opt.opt.master[here].bfloat16())
+        checked += b - a
+        at += -(-(b - a) // 256) * 256
+    comm.close()
+    return dict(off, checked=checked)
+
+
 def run_load(rank, world):
     """States and parameters loaded into an optimizer that was made from others: a step of an infinite
     norm leaves the parameters as they are, and the next one goes on from the loaded states."""

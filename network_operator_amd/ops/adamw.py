@@ -70,6 +70,12 @@ def _gradients(grads):
     return dtype, device, [0 if g is None else g.data_ptr() for g in grads]
 
 
+def _refuse_shared(params):
+    held = sorted((p.data_ptr(), p.numel() * p.element_size()) for p in params if p.numel())
+    if any(a + n > b for (a, n), (b, _) in zip(held, held[1:])):
+        raise ValueError("two parameters share memory")
+
+
 def _one(t, dtype, device, what):
     if t.dtype != dtype or t.numel() != 1:
         raise ValueError(f"{what}: expected one {dtype} element")
@@ -177,9 +183,7 @@ class AdamW:
                 raise ValueError(f"parameters must have one type: {self.dtype} and {p.dtype}")
             if not p.is_contiguous():
                 raise ValueError("parameters must be contiguous")
-        held = sorted((p.data_ptr(), p.numel() * p.element_size()) for p in self.params if p.numel())
-        if any(a + n > b for (a, n), (b, _) in zip(held, held[1:])):
-            raise ValueError("two parameters share memory")
+        _refuse_shared(self.params)
         if not all(p.is_cuda and p.device == self.device for p in self.params):
             raise ValueError("every tensor must be on one CUDA device")
         self.lr, self.betas, self.eps, self.weight_decay = float(lr), tuple(betas), float(eps), float(weight_decay)

@@ -42,6 +42,7 @@ class ShardedAdamW:
         for p in self.params:
             if p.dtype != torch.bfloat16 or not p.is_contiguous() or p.device != comm.device:
                 raise ValueError("expected contiguous bfloat16 parameters on the communicator's device")
+        A._refuse_shared(self.params)
         if max_norm is not None and not max_norm >= 0:
             raise ValueError("max_norm must not be negative")
         self.offsets, total = [], 0

@@ -82,3 +82,16 @@ def test_sharded_steps_are_clipped_averaged_and_decayed(cuda_device, world):
     for r in rows:
         assert r["exp_avg"] <= 4 and r["exp_avg_sq"] <= 0.1 and r["master"] <= 225 and r["parameters"] == 0, r
     assert sum(r["checked"] for r in rows) == 33 * 5 + 1000 + 7 + 64 * 64, rows
+
+
+def test_sharded_adamw_refuses_parameters_that_share_memory():
+    """A tied weight given twice: its gradient would count twice in the norm, and two masters would drift apart."""
+    from network_operator_amd.parallel.sharded_adamw import ShardedAdamW
+
+    class Comm:
+        rank, world, device = 0, 2, torch.device("cpu")
+
+    p = torch.zeros(16, dtype=torch.bfloat16)
+    for pair in ([p, p], [p[:9], p[8:]]):
+        with pytest.raises(ValueError, match="share memory"):
+            ShardedAdamW(Comm(), pair, lr=1e-3)

@@ -130,6 +130,7 @@ def grad_norm(grads, total, *, norms=None, coef=None, max_norm=None, scale=1.0) 
     if rc == _OVERLAP:
         raise ValueError("total, norms and coef must not share memory with each other or a gradient")
     hip._check(rc, "netop_grad_norm")
+    hip._written([t for t in (total, norms, coef) if t is not None])
 
 
 class AdamW:
@@ -207,6 +208,7 @@ class AdamW:
             self.master = torch.zeros(total, **new)
             for p, at, n in zip(self.params, self.offsets, ns):
                 self.master[at:at + n].copy_(p.detach().reshape(-1))
+        self._states = [t for t in self.state_dict().values() if t is not None]
         self._plan(ns)
 
     def _plan(self, ns):
@@ -304,3 +306,5 @@ class AdamW:
                                self.exp_avg_sq_scale.data_ptr() if eight else 0, coef_ptr, on_device, *hyper, n,
                                self._kind, _KINDS[gtype], self.state_bits, b - a, device)
             hip._check(L.netop_adamw_step(block, at + 8 * a, stream), "netop_adamw_step")
+        given = self.params if 0 not in ptrs else [p for p, g in zip(self.params, grads) if g is not None]
+        hip._written([*given, *self._states])

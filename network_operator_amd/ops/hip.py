@@ -10,6 +10,7 @@ from __future__ import annotations
 
 import ctypes
 import threading
+from operator import attrgetter
 
 from ..utils.paths import hip_library, native_bin
 
@@ -105,6 +106,34 @@ def _raw_stream(device: int) -> int:
     import torch
 
     return torch._C._cuda_getCurrentRawStream(device)
+
+
+_requires_grad = attrgetter("requires_grad")
+
+
+def _refuse_grad(tensors) -> None:
+    """What writes into given tensors is no part of a graph: the gradient would be lost without a word."""
+    if True in map(_requires_grad, tensors):
+        import torch
+
+        if torch.is_grad_enabled():
+            raise ValueError("automatic differentiation: a tensor of the call requires grad, and the call is no part of "
+                             "a graph (make it under torch.no_grad() or in the passes of an autograd.Function)")
+
+
+_increment_version = None
+
+
+def _written(tensors) -> None:
+    """Raises the version counters of tensors that a kernel writes: a graph that has kept one of them
+    refuses its backward pass instead of reading the new values.  What
+    torch.autograd.graph.increment_version does, 0.3 us sooner."""
+    global _increment_version
+    if _increment_version is None:
+        import torch
+
+        _increment_version = torch._C._increment_version
+    _increment_version(tensors)
 
 
 def _check_buf(t):

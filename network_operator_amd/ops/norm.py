@@ -12,11 +12,15 @@ front of the next product.  :func:`add_rms_norm` does all three in one pass over
 Every entry point runs on the tensors' device and that device's current stream, writes into tensors
 that the caller allocated, and raises if the library is missing.  Nothing is synchronised, allocated
 on the host or kept between calls, so the calls can be captured into a graph.
+
+None is part of an autograd graph: with grad mode on, tensors that require grad are refused.  In an
+``autograd.Function`` the first is the forward pass and the second the backward one.
 """
 
 from __future__ import annotations
 
 import struct
+from operator import methodcaller
 
 from . import hip
 
@@ -71,10 +75,12 @@ def _flat(t, shape, dtype, other, what):
         raise ValueError(f"{what}: must be contiguous")
 
 
+_device = methodcaller("get_device")
+
+
 def _on_one_device(device, tensors):
-    for t in tensors:
-        if t.get_device() != device or device < 0:
-            raise ValueError("every tensor must be on one CUDA device")
+    if device < 0 or set(map(_device, tensors)) != {device}:
+        raise ValueError("every tensor must be on one CUDA device")
 
 
 def _failed(rc, what):
@@ -111,6 +117,7 @@ def add_rms_norm(srcs, weight, out, *, residual=None, residual_out=None, rstd=No
     args = _arguments(srcs, weight, out, residual, residual_out, rstd, scales, eps)
     if args:
         _launch(*args)
+        hip._written([t for t in (out, residual_out, rstd, scales) if t is not None])
 
 
 def _arguments(srcs, weight, out, residual, residual_out, rstd, scales, eps):
@@ -136,10 +143,10 @@ def _arguments(srcs, weight, out, residual, residual_out, rstd, scales, eps):
     elif scales is not None:
         raise ValueError("scales belong to an e4m3 output")
     out_pitch = _pitch(out, shape, e4m3 if kind else dtype, "out", True)
-    tensors = [*srcs, weight]
+    tensors = [*srcs, weight, out]
     first, strides = _pitch(srcs[0], shape, dtype, "partial sum"), srcs[0].stride()
-    pitches = [first if t.dtype is dtype and t.shape == shape and t.stride() == strides else
-               _pitch(t, shape, dtype, "partial sum") for t in srcs]  # most are alike
+    pitches = [first, *[first if t.dtype is dtype and t.shape == shape and t.stride() == strides else
+                        _pitch(t, shape, dtype, "partial sum") for t in srcs[1:]]]  # most are alike
     ptrs = [t.data_ptr() for t in srcs]
     if residual is not None:
         pitches.append(_pitch(residual, shape, dtype, "residual"))
@@ -155,6 +162,7 @@ def _arguments(srcs, weight, out, residual, residual_out, rstd, scales, eps):
         tensors.append(rstd)
     if scales_ptr:
         tensors.append(scales)
+    hip._refuse_grad(tensors)
     _on_one_device(device, tensors)
     rows = out.numel() // cols
     if not rows:
@@ -203,9 +211,10 @@ def add_rms_norm_backward(dy, h, weight, rstd, dh, dweight, *, dresidual=None) -
     _flat(weight, (cols,), dtype, f32, "weight")
     _flat(rstd, shape[:-1], f32, f32, "rstd")
     _flat(dweight, (cols,), weight.dtype, f32, "dweight")
-    tensors = [h, weight, rstd, dh, dweight]
+    tensors = [dy, h, weight, rstd, dh, dweight]
     if dresidual is not None:
         tensors.append(dresidual)
+    hip._refuse_grad(tensors)
     _on_one_device(device, tensors)
     L = hip._lib or hip.lib()
     parts = L.netop_norm_backward_parts(rows, cols)
@@ -217,3 +226,4 @@ def add_rms_norm_backward(dy, h, weight, rstd, dh, dweight, *, dresidual=None) -
     rc = L.netop_add_rms_norm_backward(block, hip._raw_stream(device))
     if rc:
         _failed(rc, "netop_add_rms_norm_backward")
+    hip._written((dh, dweight))

@@ -269,6 +269,7 @@ class XgmiAllReduce:
             N._launch(*args)
         finally:  # also of a call that is refused: the peers wait here, and would take the next call's barrier for it
             self._sync_and_wait(stream)  # nobody reads my partial sum any more
+        H._written([t for t in (out, residual_out, rstd, scales) if t is not None])
 
     def reduce_scatter(self, numel: int, offset: int = 0):
         """Rank d gets chunk d of the sum of every rank's ``input(offset + numel)[offset:]``

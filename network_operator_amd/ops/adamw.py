@@ -208,7 +208,9 @@ class AdamW:
             self.master = torch.zeros(total, **new)
             for p, at, n in zip(self.params, self.offsets, ns):
                 self.master[at:at + n].copy_(p.detach().reshape(-1))
-        self._states = [t for t in self.state_dict().values() if t is not None]
+        self._sizes = torch.tensor(ns, device="cpu")
+        self._states = [t for t in (self.exp_avg, self.exp_avg_sq, self.master, self.exp_avg_scale, self.exp_avg_sq_scale)
+                        if t is not None]
         self._plan(ns)
 
     def _plan(self, ns):
@@ -231,14 +233,18 @@ class AdamW:
                           for a in range(0, len(ns), most) for b in (min(a + most, len(ns)),)]
 
     def state_dict(self) -> dict:
-        """The states themselves (not copies); ``None`` for those this optimizer has not."""
+        """The states themselves (not copies), ``None`` for those this optimizer has not, and the tensors'
+        ``sizes`` (int64, on the CPU)."""
         return dict(exp_avg=self.exp_avg, exp_avg_sq=self.exp_avg_sq, master=self.master,
-                    exp_avg_scale=self.exp_avg_scale, exp_avg_sq_scale=self.exp_avg_sq_scale)
+                    exp_avg_scale=self.exp_avg_scale, exp_avg_sq_scale=self.exp_avg_sq_scale, sizes=self._sizes)
 
     def load_state_dict(self, state: dict) -> None:
-        """Copies states in that :meth:`state_dict` of an optimizer over tensors of these sizes gave;
-        the parameters are not touched."""
+        """Copies states in that :meth:`state_dict` of an optimizer over tensors of these sizes gave
+        (where they have no ``sizes``, only the padded total is compared); the parameters are not touched."""
         mine = self.state_dict()
+        sizes = mine.pop("sizes")
+        if state.get("sizes") is not None and state["sizes"].tolist() != sizes.tolist():
+            raise ValueError("states of tensors of other sizes")
         for k, t in mine.items():
             x = state.get(k)
             if (x is None) != (t is None) or t is not None and (x.shape != t.shape or x.dtype != t.dtype):

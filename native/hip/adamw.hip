@@ -25,6 +25,8 @@
 // third of sqrt(v) -- of each element on its own, around the right mean.
 #include "elem.hpp"
 
+#include <algorithm>
+
 using namespace netop;
 
 namespace {
@@ -355,29 +357,58 @@ __global__ __launch_bounds__(kFinalThreads) void sumsq_final_kernel(NormGroup gr
 
 constexpr int kOverlap = -1;  // ops/adamw.py raises ValueError for it
 
+// What a step writes, as packed by ops/adamw.py:_HELD: spans that do not overlap, by address.
+struct Span {
+    uint64_t from, to;
+    int64_t owner;  // the parameter that it is, or -1
+};
+struct Held {
+    const Span* spans;
+    const uint64_t* elements;  // of each gradient
+    int64_t n_spans, n;
+};
+
+// Whether a gradient (coef) lies in a span, except a gradient in its own parameter's, element on element.
+bool strays(const Held& held, const void* const* grads, uint64_t size, uint64_t own_size, const float* coef) {
+    const Span* end = held.spans + held.n_spans;
+    for (int64_t i = 0; i <= held.n; ++i) {
+        const bool is_coef = i == held.n;
+        const auto at = reinterpret_cast<uintptr_t>(is_coef ? coef : grads[i]);
+        const uint64_t bytes = is_coef ? 4 : held.elements[i] * size;
+        if (!at || !bytes) continue;
+        const Span* s = std::upper_bound(held.spans, end, uint64_t(at), [](uint64_t x, const Span& y) { return x < y.to; });
+        if (s == end || s->from >= at + bytes) continue;  // the first that ends behind `at`
+        if (is_coef || s->owner != i || s->from != at || size != own_size) return true;
+    }
+    return false;
+}
+
 }  // namespace
 
 extern "C" {
 
-// Return hipError_t values (0 = success).
+// Return hipError_t values (0 = success), or -1 for tensors that may not share memory.
 
 int netop_adamw_chunk() { return kChunk; }
 int netop_adamw_max_grads() { return kMaxGrads; }
 int netop_adamw_hyper_bytes() { return int(sizeof(Hyper)); }
 
-// One launch over p->n_chunks chunks, whose tensors' gradients are grads[0 .. n_grads).
-int netop_adamw_step(const StepParams* p, const void* const* grads, hipStream_t stream) {
-    if (!p || !grads || p->n_grads < 1 || p->n_grads > kMaxGrads || p->n_chunks < 0 || !p->m || !p->v ||
+// One launch over p->n_chunks chunks, whose tensors' gradients are grads[first .. first + n_grads).  With
+// `held` every one of its n gradients and coef are looked up first: a gradient may lie where its own
+// parameter does, element on element, and nowhere else that a step writes.
+int netop_adamw_step(const StepParams* p, const void* const* grads, int first, const Held* held, hipStream_t stream) {
+    if (!p || !grads || first < 0 || p->n_grads < 1 || p->n_grads > kMaxGrads || p->n_chunks < 0 || !p->m || !p->v ||
         (p->bits != 8 && p->bits != 32) || (p->bits == 8 && (!p->m_scale || !p->v_scale)) ||
         (p->ptype != kF32 && !p->master))
         return int(hipErrorInvalidValue);
     if (p->n_chunks == 0) return int(hipSuccess);
     // A grid's threads are counted in 32 bits.
     if (!p->chunks || uint64_t(p->n_chunks) * kThreads > 0xffffffffu) return int(hipErrorInvalidValue);
+    if (held && strays(*held, grads, p->gtype == kF32 ? 4 : 2, p->ptype == kF32 ? 4 : 2, p->coef)) return kOverlap;
     const OnDevice on(p->device);
     if (on.err != hipSuccess) return int(on.err);
     Grads g;
-    for (int i = 0; i < kMaxGrads; ++i) g.at[i] = i < p->n_grads ? grads[i] : nullptr;
+    for (int i = 0; i < kMaxGrads; ++i) g.at[i] = i < p->n_grads ? grads[first + i] : nullptr;
     bool known = false;
     switch (p->ptype) {
         case kF32: known = launch_grads<float>(*p, g, stream); break;

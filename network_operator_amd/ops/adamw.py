@@ -27,7 +27,8 @@ from . import hip
 
 BLOCK = 256  # elements of a tensor that share a scale; every tensor's states start at a whole block
 
-# native/hip/adamw.hip:Hyper and StepParams
+# native/hip/adamw.hip:Hyper, StepParams and Held
+_HELD = struct.Struct("=2Q2q")
 _HYPER = struct.Struct("=9fI")
 _STEP = struct.Struct("=8Q" + "9fI" + "6i")
 _OVERLAP = -1
@@ -227,6 +228,11 @@ class AdamW:
         start = (torch.arange(firsts[-1], device=self.device) - rows[3][of]) * chunk
         self._table = torch.stack([rows[0][of] + start * self.params[0].element_size(), rows[1][of] + start, start,
                                    (rows[2][of] - start).clamp(max=chunk) | (of % most) << 32], 1)
+        # What a step writes: address, end, and the parameter that it is.
+        spans = sorted((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size(), i)
+                       for i, t in [*enumerate(self.params), *((-1, t) for t in self._states)] if t.numel())
+        self._spans, self._elements = array("q", [x for s in spans for x in s]), array("Q", ns)
+        self._held = _HELD.pack(self._spans.buffer_info()[0], self._elements.buffer_info()[0], len(spans), len(ns))
         # (first tensor, one behind the last, address of its chunks, how many)
         at = self._table.data_ptr()
         self._launches = [(a, b, at + 32 * firsts[a], firsts[b] - firsts[a])
@@ -257,7 +263,8 @@ class AdamW:
     def step(self, grads, *, step, lr=None, coef=None, scale=1.0) -> None:
         """One step from ``grads``, one a parameter: contiguous, of its shape, all of one type (fp32,
         bf16 or fp16).  A parameter whose gradient is ``None`` is left as it is, with its states.  A
-        gradient may be its own parameter's memory, but no other tensor's of this optimizer.
+        gradient may be its own parameter's memory, element on element, but no other tensor's of this
+        optimizer, and nor may ``coef``.
 
         ``step`` counts from 1: a number, or an int64 tensor of one element on the device (one below
         1 is taken for 1 there).  ``lr``
@@ -303,7 +310,7 @@ class AdamW:
                                            lr_ptr, step_ptr, t, device, stream), "netop_adamw_hyper")
         eight = self.state_bits == 8
         table = array("Q", ptrs)
-        at = table.buffer_info()[0]
+        at, held = table.buffer_info()[0], self._held
         for a, b, chunks, n in self._launches:
             if n == 0:
                 continue  # nothing but empty tensors
@@ -311,6 +318,11 @@ class AdamW:
                                self.exp_avg_sq.data_ptr(), self.exp_avg_scale.data_ptr() if eight else 0,
                                self.exp_avg_sq_scale.data_ptr() if eight else 0, coef_ptr, on_device, *hyper, n,
                                self._kind, _KINDS[gtype], self.state_bits, b - a, device)
-            hip._check(L.netop_adamw_step(block, at + 8 * a, stream), "netop_adamw_step")
+            rc = L.netop_adamw_step(block, at, a, held, stream)
+            if rc == _OVERLAP:
+                raise ValueError("a gradient or coef lies in the memory of another tensor of this optimizer (a gradient "
+                                 "may be its own parameter's memory, element on element)")
+            hip._check(rc, "netop_adamw_step")
+            held = None  # all of them have been looked up
         given = self.params if 0 not in ptrs else [p for p, g in zip(self.params, grads) if g is not None]
         hip._written([*given, *self._states])

@@ -79,7 +79,7 @@ def lib() -> ctypes.CDLL:
             L.netop_add_rms_norm_backward.restype = i32
             for f in (L.netop_adamw_chunk, L.netop_adamw_max_grads, L.netop_adamw_hyper_bytes):
                 f.argtypes, f.restype = [], i32
-            L.netop_adamw_step.argtypes = [block, vp, vp]
+            L.netop_adamw_step.argtypes = [block, vp, i32, block, vp]
             L.netop_adamw_step.restype = i32
             L.netop_adamw_hyper.argtypes = [vp, block, f64, f64, f64, f64, u32, vp, vp, i64, i32, vp]
             L.netop_adamw_hyper.restype = i32

@@ -350,7 +350,7 @@ __global__ __launch_bounds__(kFinalThreads) void sumsq_final_kernel(NormGroup gr
         *a.total = float(total);
         if (a.coef) {
             const double clip = double(a.max_norm) / (total + 1e-6);
-            *a.coef = float(double(a.scale) * (total < __builtin_inf() ? (clip < 1 ? clip : 1.0) : __builtin_nan("")));
+            *a.coef = float(double(a.scale) * (float(total) < __builtin_inff() ? (clip < 1 ? clip : 1.0) : __builtin_nan("")));
         }
     }
 }

@@ -92,9 +92,9 @@ def grad_norm(grads, total, *, norms=None, coef=None, max_norm=None, scale=1.0) 
     ``total`` (fp32, one element) takes the norm; ``norms`` (fp32, one a gradient), where given, each
     gradient's own, times ``scale`` too; ``coef`` (fp32, one element), where given,
     ``scale * min(1, max_norm / (total + 1e-6))``, the factor :meth:`AdamW.step` takes (``scale``
-    without ``max_norm``).  Where the norm is infinite or NaN ``coef`` is NaN, and that step is left out.
+    without ``max_norm``).  Where ``total`` is infinite (in fp32) or NaN ``coef`` is NaN, and that step is left out.
 
-    Squares are summed in 64 bits, in an order that depends on the sizes alone: no gradient is too
+    Squares are summed in 64 bits, in an order that depends on the sizes alone: no square is too
     large or too small, and the same inputs give the same bits.
     """
     import torch

@@ -1,4 +1,6 @@
-"""States and gradients that do not belong to an optimizer's tensors (ops/adamw.py)."""
+"""States, gradients and norms that an optimizer cannot take (ops/adamw.py)."""
+
+import math
 
 import pytest
 
@@ -75,3 +77,15 @@ def test_views_between_the_parameters_are_taken(cuda_device):
     opt.step([buf[900:1200], buf[900:1200], buf[620:620]], step=2)
     torch.cuda.synchronize()
     assert bool((buf[:300] < 0).all()) and bool((buf[600:900] < 0).all()) and bool((buf[300:600] == 0).all())
+
+
+@pytest.mark.gpu
+def test_a_norm_beyond_fp32_leaves_the_step_out(cuda_device):
+    """Finite in 64 bits, infinite as the fp32 total: the factor is NaN, as for any infinite norm."""
+    g = torch.full((1000,), 3e38, device=cuda_device)
+    total, coef = torch.zeros(1, device=cuda_device), torch.zeros(1, device=cuda_device)
+    adamw.grad_norm([g], total, coef=coef, max_norm=1.0)
+    assert float(total) == math.inf and math.isnan(float(coef))
+    adamw.grad_norm([g], total, coef=coef, max_norm=1.0, scale=2.0 ** -10)
+    want = 2.0 ** -10 * float(g[0]) * math.sqrt(1000)
+    assert float(total) == pytest.approx(want, rel=2 ** -22) and float(coef) == pytest.approx(2.0 ** -10 / want, rel=1e-6, abs=2e-45)

@@ -73,6 +73,9 @@ static_assert(sizeof(StepParams) == 128 && sizeof(Hyper) == 40 && sizeof(Chunk) 
 static_assert(sizeof(StepParams) + sizeof(Grads) <= 4096, "kernel arguments");
 
 // Four random numbers, for the positions from a multiple of four on: one product reaches all of them.
+// The two rounds of xor-shift and product are the 32-bit mixer of C. Wellons, "Prospecting for Hash
+// Functions" (2018); the odd constants that spread position, seed and step come from the public-domain
+// hashes of A. Appleby and Y. Collet, where any odd numbers of mixed bits would do.
 __device__ __forceinline__ Vec<uint32_t, 4> random4(uint64_t position, uint32_t key) {
     constexpr uint32_t kLow = 0x9E3779B1u;
     const uint32_t low = uint32_t(position) * kLow, high = uint32_t(position >> 32) * 0x85EBCA77u ^ key;

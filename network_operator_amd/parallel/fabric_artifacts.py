@@ -70,6 +70,19 @@ def _sha256(path: str) -> Optional[str]:
         return None
 
 
+def pci_netdevs(sysfs_root: str = "/sys") -> List[str]:
+    """The netdevs that are PCI network functions of this node, from sysfs alone.  Without one (a
+    virtual machine that was given the GPU only) there is nothing to discover, and the agent says so
+    and fails, as it does on any node where it finds no interface."""
+    def read(path: Path) -> str:
+        try:
+            return path.read_text().strip()
+        except OSError:
+            return ""
+
+    return sorted(d.name for d in Path(sysfs_root, "class/net").glob("*") if read(d / "device" / "class").startswith("0x02"))
+
+
 def generate(out_dir: str, sysfs_root: Optional[str] = None, env_extra: str = "", timeout: float = 60) -> dict:
     """Runs ``discover --dry-run`` into ``out_dir``; returns the artifacts' description:
     ``{"applied": False, "env": {...}, "topo_file", "topo_file_bytes", "topo_sha256", "agent_ms",

@@ -23,9 +23,21 @@ def _netns_ok():
         return False, str(e)
 
 
+# What these test on the node itself is its scale-out NICs (discovery, their place in RCCL's topology).
+NEEDS_NICS = {"test_agent_dry_run_on_this_node", "test_node_report_on_this_node", "test_topo_tool_on_this_node",
+              "test_require_rdma_dry_run_on_this_node_names_every_rail_without_an_rdma_device",
+              "test_fabric_validation_single_gpu", "test_rccl_loads_generated_topology",
+              "test_bench_measures_with_the_agents_file_and_reads_rccl_dump"}
+
+
 def pytest_collection_modifyitems(config, items):
+    from network_operator_amd.parallel.fabric_artifacts import pci_netdevs
+
     ok, why = None, None
+    without_nics = not pci_netdevs(os.environ.get("SYSFS_ROOT", "/sys"))
     for item in items:
+        if without_nics and item.name in NEEDS_NICS:
+            item.add_marker(pytest.mark.skip(reason="this node has no NIC: no netdev is a PCI network function"))
         if "netns" in item.keywords:
             if ok is None:
                 ok, why = _netns_ok()

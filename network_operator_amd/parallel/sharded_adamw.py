@@ -29,8 +29,8 @@ class ShardedAdamW:
     constructor takes rank 0's layout for granted and every rank's values for equal).  Gradients are
     averaged over the ranks, in bf16 as they cross the links; masters and states are fp32, or 8-bit
     states (:class:`~network_operator_amd.ops.adamw.AdamW`, whose options these are), whose blocks start
-    where a rank's part of a parameter does.  With ``max_norm`` gradients are clipped by the norm of all of them; a step whose norm is infinite or
-    NaN changes nothing on any rank."""
+    where a rank's part of a parameter does.  With ``max_norm`` gradients are clipped by the norm of all
+    of them; a step whose norm is infinite or NaN changes nothing on any rank."""
 
     def __init__(self, comm: XgmiAllReduce, params, *, lr, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.01,
                  state_bits=32, seed=0, max_norm=None):
@@ -69,8 +69,8 @@ class ShardedAdamW:
         self._sizes = self._sizes or [0, 0]
         self._sizes.append(self.chunk - end)
         # every rank its own random numbers: the chunks' positions all start at zero
-        self.opt = A.AdamW(self._parts(self.shard), lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, state_bits=state_bits,
-                           seed=(seed + 0x9E3779B1 * comm.rank) % (1 << 32))
+        self.opt = A.AdamW(self._parts(self.shard), lr=lr, betas=betas, eps=eps, weight_decay=weight_decay,
+                           state_bits=state_bits, seed=(seed + 0x9E3779B1 * comm.rank) % (1 << 32))
         self._norm, self._coef = (torch.empty(1, device=comm.device) for _ in range(2))
 
     def _parts(self, chunk):

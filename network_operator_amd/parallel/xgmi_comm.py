@@ -122,7 +122,7 @@ class XgmiAllReduce:
         if not 1 <= self.world <= MAX_RANKS:
             raise ValueError(f"1..{MAX_RANKS} ranks (one node) supported, got {self.world}")
         self.device = torch.device(device if device is not None else "cuda")
-        if self.device.index is None:  # "cuda" is not equal to the device of a tensor on it
+        if self.device.type == "cuda" and self.device.index is None:  # "cuda" is not equal to the device of a tensor on it
             self.device = torch.device("cuda", torch.cuda.current_device())
         self.timeout_s = timeout_s
         self.wg_per_cu = wg_per_cu

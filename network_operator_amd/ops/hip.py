@@ -10,7 +10,6 @@ from __future__ import annotations
 
 import ctypes
 import threading
-from operator import attrgetter
 
 from ..utils.paths import hip_library, native_bin
 
@@ -100,40 +99,35 @@ def _stream(tensor):
     return ctypes.c_void_p(torch.cuda.current_stream(tensor.device).cuda_stream)
 
 
+_C = None  # torch._C, once torch is there; the three calls below are in every operator's way
+
+
+def _torch():
+    global _C
+    import torch
+
+    _C = torch._C
+    return _C
+
+
 def _raw_stream(device: int) -> int:
     """The current stream of device ``device`` as an address.  What torch.cuda.current_stream(...)
     .cuda_stream gives, without its two objects: 0.1 against 2.1 us, a fifth of a small call."""
-    import torch
-
-    return torch._C._cuda_getCurrentRawStream(device)
-
-
-_requires_grad = attrgetter("requires_grad")
+    return (_C or _torch())._cuda_getCurrentRawStream(device)
 
 
 def _refuse_grad(tensors) -> None:
     """What writes into given tensors is no part of a graph: the gradient would be lost without a word."""
-    if True in map(_requires_grad, tensors):
-        import torch
-
-        if torch.is_grad_enabled():
-            raise ValueError("automatic differentiation: a tensor of the call requires grad, and the call is no part of "
-                             "a graph (make it under torch.no_grad() or in the passes of an autograd.Function)")
-
-
-_increment_version = None
+    if (_C or _torch())._any_requires_grad(*tensors) and _C.is_grad_enabled():
+        raise ValueError("automatic differentiation: a tensor of the call requires grad, and the call is no part of a "
+                         "graph (make it under torch.no_grad() or in the passes of an autograd.Function)")
 
 
 def _written(tensors) -> None:
     """Raises the version counters of tensors that a kernel writes: a graph that has kept one of them
     refuses its backward pass instead of reading the new values.  What
     torch.autograd.graph.increment_version does, 0.3 us sooner."""
-    global _increment_version
-    if _increment_version is None:
-        import torch
-
-        _increment_version = torch._C._increment_version
-    _increment_version(tensors)
+    (_C or _torch())._increment_version(tensors)
 
 
 def _check_buf(t):

@@ -149,7 +149,8 @@ def _arguments(srcs, weight, out, residual, residual_out, rstd, scales, eps):
                         _pitch(t, shape, dtype, "partial sum") for t in srcs[1:]]]  # most are alike
     ptrs = [t.data_ptr() for t in srcs]
     if residual is not None:
-        pitches.append(_pitch(residual, shape, dtype, "residual"))
+        pitches.append(first if residual.dtype is dtype and residual.shape == shape and residual.stride() == strides else
+                       _pitch(residual, shape, dtype, "residual"))
         ptrs.append(residual.data_ptr())
         tensors.append(residual)
     if residual_out is not None:

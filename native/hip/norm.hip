@@ -156,6 +156,13 @@ __device__ __forceinline__ Vec<float, 8> weights8(const void* w, int f32, int c)
 // The larger of two magnitudes; NaN stays.
 __device__ __forceinline__ float larger(float x, float y) { return x > y || x != x ? x : y; }
 
+// What values up to amax are stored with, and the factor of their codes: the reciprocal of the scale as it
+// is stored, so that code x scale is nearest by that scale.
+__device__ __forceinline__ void scale_of(float amax, float& scale, float& inv) {
+    scale = amax < kTiny ? 0.0f : amax / kE4m3Max;
+    inv = amax < kTiny ? 0.0f : 1.0f / scale;
+}
+
 // AHEAD inputs are on their way together: with peer pointers each is an xGMI round trip.
 template <class T, int TPR, int VPT, int AHEAD, bool E4M3, bool WHOLE, bool STREAM>
 __global__ __launch_bounds__(Threads<TPR>::kBlock) void norm_kernel(NormParams a) {
@@ -220,9 +227,11 @@ __global__ __launch_bounds__(Threads<TPR>::kBlock) void norm_kernel(NormParams a
         uint8_t* p = static_cast<uint8_t*>(a.out) + int64_t(row) * a.out_stride;
         const bool by_group = a.out_kind == kGroupScale;
         const int groups = (cols + kGroup - 1) / kGroup;
+        float scale = 0, inv = 0;
         if (!by_group) {
             amax = row_max<TPR>(amax, red[1]);
-            if (t == 0 && here) a.scales[row] = amax < kTiny ? 0.0f : amax / kE4m3Max;
+            scale_of(amax, scale, inv);
+            if (t == 0 && here) a.scales[row] = scale;
         }
 #pragma unroll
         for (int k = 0; k < VPT; ++k) {
@@ -232,9 +241,9 @@ __global__ __launch_bounds__(Threads<TPR>::kBlock) void norm_kernel(NormParams a
 #pragma unroll
                 for (int j = 0; j < 8; ++j) amax = j >= at.twice ? larger(amax, fabsf(h[k][j])) : amax;
                 amax = lanes_max<(TPR == 8 ? 8 : 16), true>(amax);
-                if ((t & 15) == 0 && at.in) a.scales[row * groups + (k * n + t) / 16] = amax < kTiny ? 0.0f : amax / kE4m3Max;
+                scale_of(amax, scale, inv);
+                if ((t & 15) == 0 && at.in) a.scales[row * groups + (k * n + t) / 16] = scale;
             }
-            const float inv = amax < kTiny ? 0.0f : 1.0f / (amax / kE4m3Max);  // of the scale as it is stored
             if (!at.in) continue;
             Vec<float, 8> q;
 #pragma unroll
@@ -279,8 +288,9 @@ __global__ __launch_bounds__(256) void narrow_norm_kernel(NormParams a) {
             y[c] = h[c] * rstd * (a.weight_f32 ? static_cast<const float*>(a.weight)[c] : float(static_cast<const T*>(a.weight)[c]));
             amax = larger(amax, fabsf(y[c]));
         }
-    const float inv = amax < kTiny ? 0.0f : 1.0f / (amax / kE4m3Max);  // of the scale as it is stored
-    if (a.out_kind != kSame) a.scales[row] = amax < kTiny ? 0.0f : amax / kE4m3Max;
+    float scale, inv;
+    scale_of(amax, scale, inv);
+    if (a.out_kind != kSame) a.scales[row] = scale;
 #pragma unroll
     for (int c = 0; c < 7; ++c)
         if (c < a.cols) {

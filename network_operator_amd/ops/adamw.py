@@ -212,6 +212,7 @@ class AdamW:
         self._sizes = torch.tensor(ns, device="cpu")
         self._states = [t for t in (self.exp_avg, self.exp_avg_sq, self.master, self.exp_avg_scale, self.exp_avg_sq_scale)
                         if t is not None]
+        self._all = [*self.params, *self._states]
         self._plan(ns)
 
     def _plan(self, ns):
@@ -324,5 +325,5 @@ class AdamW:
                                  "may be its own parameter's memory, element on element)")
             hip._check(rc, "netop_adamw_step")
             held = None  # all of them have been looked up
-        given = self.params if 0 not in ptrs else [p for p, g in zip(self.params, grads) if g is not None]
-        hip._written([*given, *self._states])
+        hip._written(self._all if 0 not in ptrs else
+                     [*(p for p, g in zip(self.params, grads) if g is not None), *self._states])

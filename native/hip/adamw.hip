@@ -16,8 +16,8 @@
 // m that is not would make the next update m / eps.
 //
 // Bound by HBM: with a bf16 gradient and parameter and an fp32 master 28 bytes an element, 16 with states in
-// 8 bits.  2^29 elements of the one take 2.7 ms (5.6 TB/s, a large copy's rate), 2^28 of the other 0.73 ms
-// (5.9 TB/s).  The 8-bit states' arithmetic comes near that too, some 100 instructions an element: before the
+// 8 bits.  2^29 elements of the one take 2.7 ms (5.6 TB/s, a large copy's rate), 2^28 of the other 0.74 ms
+// (5.8 TB/s).  The 8-bit states' arithmetic comes near that too, some 100 instructions an element: before the
 // bounds checks left whole chunks and the divisions the step it took 0.80 ms.
 //
 // What stochastic rounding costs: a value that moves by D times itself carries a noise of about the root
@@ -33,7 +33,7 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kBlock = 256;          // elements that share a scale: 64 lanes x 4
-constexpr int kUnroll = 2;           // blocks a wavefront works on together: 4 leave uneven ends (784 us for 755)
+constexpr int kUnroll = 2;           // blocks a wavefront works on together: 4 leave uneven ends (2^28 elements: 4 % slower)
 constexpr int kChunk = kThreads / 64 * kUnroll * kBlock;  // elements of one workgroup
 constexpr int kMaxGrads = 440;       // gradient addresses that fit a launch's arguments (4 KiB)
 
@@ -265,7 +265,9 @@ bool launch_grads(const StepParams& a, const Grads& g, hipStream_t stream) {
 // Sums of squares in 64 bits throughout: squares of fp32 gradients leave fp32's range long before
 // the gradients do, and 2^29 terms its precision.  A workgroup sums one stretch of one tensor; a
 // second launch of one workgroup adds up the stretches in a fixed order.  Bound by HBM reads: 1 GiB of
-// bf16 takes 177 us (6.1 TB/s); 2^20 fp32 elements 4.2 + 2.8 us, less than the host takes to ask for them.
+// bf16 in 290 tensors takes 177 us (6.1 TB/s); 2^20 fp32 elements in 23 4.1 + 2.7 us, less than the host takes to
+// ask for them.  Eight lanes add up a tensor's stretches, which a single large tensor waits for: 2^27 elements of one
+// take 124 us, 2^24 49 us.
 constexpr int kMaxNormTensors = 150;  // addresses and sizes that fit a launch's arguments
 constexpr int kFinalThreads = 1024;
 

@@ -11,14 +11,15 @@
 //
 // A row of h stays in the registers of a workgroup, or of a part of a wavefront, so every input is read
 // once and every output written once.  Bound by HBM, the arithmetic is about ten operations an element:
-// 16384 x 8192 bf16 with a residual to e4m3 takes 170 us (5.5 TB/s, a large copy's rate).  Few rows are bound by
-// the way there and back: 64 x 8192 over 8 partial sums 5.8 us, one row of 4096 2.8 us.
+// 16384 x 8192 bf16 with a residual to e4m3 takes 172 us (5.5 TB/s, a large copy's rate), 8192 x 4096 fp32 97 us.
+// Few rows are bound by the way there and back: 64 x 8192 over 8 partial sums 5.8 us, one row of 4096 2.7 us.
 //
 // Backward, with x = h rstd and g = dy weight:  dh = rstd (g - x mean(g x)) + dresidual, which is the
 // gradient of every partial sum and of the residual alike; dweight = sum over rows of dy x.  x is of
 // order one whatever h is; rstd^3 would leave fp32 for rows of 1e13 or 1e-13, and dy h for others.
-// 8192 x 4096 bf16 takes 43 us and 5 us for dweight (5.5 TB/s); where rows are few and wide, one workgroup a CU
-// and the partial rows of dweight bound it: 333 x 10007 fp32 13 + 5 us, at 7 us of data.
+// 8192 x 4096 bf16 takes 44 us and 5 us for dweight (5.5 TB/s); where rows are few and wide, one workgroup a CU
+// and the partial rows of dweight bound it: 333 x 10007 fp32 13 + 5 us, at 7 us of data.  Beyond 16384 columns,
+// registers do: 3000 x 20000 bf16 135 us, at 86 us of data.
 #include "elem.hpp"
 
 using namespace netop;
@@ -493,13 +494,16 @@ struct Shape {
 
 // One vector a thread up to 4096 columns: fewest registers, most rows in flight.  Beyond, rows of two
 // vectors a thread leave each CU more workgroups (16384 x 8192 bf16 to e4m3: 176 us with 512 threads, 202 with
-// 1024), while few rows end sooner spread wider (64 x 8192, 8 partial sums: 5.0 us with 1024, 6.4 with 512).
+// 1024), while few rows end sooner spread wider.  Of calls of 64, 300, 700 and 1001 rows with 1024 / 512 threads:
+// 8192 bf16 over 8 partial sums 11.1 / 11.3, 11.5 / 11.6, 20.9 / 21.7 and 27.7 / 28.6 us, backward of 300, 700 and
+// 1001 x 5003 12.1 / 12.9, 16.0 / 17.6 and 17.8 / 20.1.  Wider loses where a second round of rows is short:
+// 1001 x 8192 of one source 13.3 / 11.5 us, 1001 x 5003 of three 12.4 / 11.7.
 Shape shape_for(int cols, uint64_t rows) {
     const int vecs = (cols + 7) / 8;
     for (int tpr = 8; tpr <= 128; tpr *= 2)
         if (vecs <= tpr) return {tpr, 1, 256};
     const int vpt = vecs <= 512 || (vecs <= 1024 && rows <= 1024) ? 1 : vecs <= 2048 ? 2 : 4;
-    // Four vectors a thread need every wavefront there is room for (backward 3000 x 20000: 142 us, 198 with 640).
+    // Four vectors a thread need every wavefront there is room for (backward 3000 x 20000: 135 us, 198 with 640).
     return {0, vpt, vpt == 4 ? 1024 : ((vecs + vpt - 1) / vpt + 63) / 64 * 64};
 }
 
